@@ -1,0 +1,260 @@
+// Fused matrix products and ragged grouped products (float64, float32): what the kernels share.
+//
+//   Z = alpha A B + bias,   C = act(Z) + beta residual
+//
+// product_tile.h holds the tiled kernel, product_rows.h the one for few rows, product.hip the
+// element-wise kernels, the choice between them and the C entry points.
+#pragma once
+#include "common.h"
+
+namespace locus {
+
+// What one element of the result goes through once its sum is there.  Strides in elements; a
+// stride of 0 broadcasts.
+struct ProductEpi {
+    void* C; long sc_m, sc_n;
+    const void* bias; long sb_m, sb_n;
+    const void* res; long sr_m, sr_n;
+    void* pre; long sp_m, sp_n;
+    double alpha, beta;
+    int act;
+};
+
+// Modes of a product: one pair of matrices; runs of rows with a B of their own; runs of the summed
+// index with a C of their own (the gradient of the runs' B).
+enum { PRODUCT_DENSE = 0, PRODUCT_ROWS = 1, PRODUCT_SUM = 2 };
+
+struct ProductDesc {
+    int m, n, k;                      // DENSE, ROWS: m = all rows; SUM: k = all rows
+    const void* A; long sa_m, sa_k;
+    const void* B; long sb_k, sb_n;
+    ProductEpi epi;
+    // runs: offsets[groups + 1] on the device, read as the largest of 0 and every earlier one and at
+    // most the number of rows, so that runs never overlap whatever the array holds
+    int groups;
+    const int64_t* offsets;
+    long sb_g, sbias_g, sc_g;         // B, bias (ROWS) and C (SUM) of the next run
+    const int64_t* gather;            // row r reads A's row gather[r]; outside [0, a_rows): NaN
+    long a_rows;
+    int fill_rest;                    // ROWS: rows of no run become 0 in C and pre
+    // a split sum: part [z][rows][n] (or [z][n][rows], following C) instead of C
+    void* part;
+    int nz, kchunk;
+    long part_m, part_n, part_z;      // strides of the partial products, in elements
+};
+
+// ---- element functions -----------------------------------------------------------------------
+// e = exp(-|z|) <= 1 carries both tails of the logistic function without overflow.
+template <class T> __device__ __forceinline__ T t_exp(T x);
+template <> __device__ __forceinline__ double t_exp(double x) { return exp(x); }
+template <> __device__ __forceinline__ float t_exp(float x) { return expf(x); }
+template <class T> __device__ __forceinline__ T t_erfc(T x);
+template <> __device__ __forceinline__ double t_erfc(double x) { return erfc(x); }
+template <> __device__ __forceinline__ float t_erfc(float x) { return erfcf(x); }
+template <class T> __device__ __forceinline__ T t_log1p(T x);
+template <> __device__ __forceinline__ double t_log1p(double x) { return log1p(x); }
+template <> __device__ __forceinline__ float t_log1p(float x) { return log1pf(x); }
+
+template <class T> __device__ __forceinline__ T logistic(T z)
+{
+    const T e = t_exp<T>(z < T(0) ? z : -z);
+    return (z < T(0) ? e : T(1)) / (T(1) + e);
+}
+template <class T> __device__ __forceinline__ T normal_cdf(T z)
+{
+    return T(0.5) * t_erfc<T>(z * T(-0.70710678118654752440));
+}
+template <class T> __device__ __forceinline__ T normal_density(T z)
+{
+    return t_exp<T>(T(-0.5) * z * z) * T(0.39894228040143267794);
+}
+// z * f where f -> 0 faster than z grows: 0 instead of inf * 0
+template <class T> __device__ __forceinline__ T times_vanishing(T z, T f)
+{
+    return f == T(0) ? T(0) : z * f;
+}
+
+template <class T> __device__ __forceinline__ T act_value(int act, T z)
+{
+    switch (act) {
+    case LOCUS_HIP_ACT_LOGISTIC: return logistic(z);
+    case LOCUS_HIP_ACT_PROBIT: return normal_cdf(z);
+    case LOCUS_HIP_ACT_SOFTPLUS:
+        return (z > T(0) ? z : T(0)) + t_log1p<T>(t_exp<T>(z < T(0) ? z : -z));
+    case LOCUS_HIP_ACT_GELU: return times_vanishing(z, normal_cdf(z));
+    case LOCUS_HIP_ACT_SILU: return times_vanishing(z, logistic(z));
+    default: return z;
+    }
+}
+
+template <class T> __device__ __forceinline__ T act_slope(int act, T z)
+{
+    switch (act) {
+    case LOCUS_HIP_ACT_LOGISTIC: {
+        const T e = t_exp<T>(z < T(0) ? z : -z);
+        return e / ((T(1) + e) * (T(1) + e));
+    }
+    case LOCUS_HIP_ACT_PROBIT: return normal_density(z);
+    case LOCUS_HIP_ACT_SOFTPLUS: return logistic(z);
+    case LOCUS_HIP_ACT_GELU: return normal_cdf(z) + times_vanishing(z, normal_density(z));
+    case LOCUS_HIP_ACT_SILU: {
+        const T s = logistic(z);
+        return s + times_vanishing(z, s * logistic(-z));
+    }
+    default: return T(1);
+    }
+}
+
+// One element of the result: `sum` is the product's, i / j its row and column, bias0 an offset of
+// the run's bias.  Reads the residual before it writes C, so that C may be the residual.
+template <class T>
+__device__ __forceinline__ void epi_store(const ProductEpi& e, long bias0, long i, long j, T sum)
+{
+    T z = T(e.alpha) * sum;
+    if (e.bias) z += static_cast<const T*>(e.bias)[bias0 + i * e.sb_m + j * e.sb_n];
+    if (e.pre) static_cast<T*>(e.pre)[i * e.sp_m + j * e.sp_n] = z;
+    T v = act_value<T>(e.act, z);
+    if (e.res) v += T(e.beta) * static_cast<const T*>(e.res)[i * e.sr_m + j * e.sr_n];
+    static_cast<T*>(e.C)[i * e.sc_m + j * e.sc_n] = v;
+}
+
+// ---- runs --------------------------------------------------------------------------------------
+struct Run {
+    int g;            // which run (-1: none)
+    long lo, hi;      // its rows (of the tile asked for)
+};
+
+__device__ __forceinline__ long uniform_long(long v)
+{
+    const int lo = __builtin_amdgcn_readfirstlane((int)(v & 0xffffffff));
+    const int hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return ((long)hi << 32) | (unsigned)lo;
+}
+
+__device__ __forceinline__ long shfl_long(long v, int lane)
+{
+    const int lo = __shfl((int)(v & 0xffffffff), lane), hi = __shfl((int)(v >> 32), lane);
+    return ((long)hi << 32) | (unsigned)lo;
+}
+
+// 64 offsets at a time, one per lane: the ordered offsets are a running maximum, the tiles before a
+// run a running sum.  Every wave does this for itself (no barrier); ~0.3 us for up to 64 runs,
+// against a launch of its own for a tile map.  `tile` counts tiles of `bm` rows over all runs in
+// order; bm = 0 looks the run of row `tile` up instead.  first / last: the rows that runs cover.
+__device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, long rows, long tile,
+                                        int bm, long* first = nullptr, long* last = nullptr)
+{
+    const int lane = threadIdx.x & 63;
+    auto bounded = [&](long v) { return v < 0 ? 0 : (v > rows ? rows : v); };
+    long carry = bounded(offsets[0]);
+    if (first) *first = carry;
+    long before = 0;                                   // tiles of the runs before this chunk
+    Run found = {-1, 0, 0};
+    for (int base = 0; base < groups; base += 64) {
+        const int g = base + lane;
+        long hi = g < groups ? bounded(offsets[g + 1]) : 0;
+        hi = hi > carry ? hi : carry;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const long o = shfl_long(hi, lane - s);
+            if (lane >= s && o > hi) hi = o;
+        }
+        const long up = shfl_long(hi, lane - 1);
+        const long lo = lane == 0 ? carry : up;
+        bool mine;
+        long excl = 0;
+        if (bm) {
+            const long t = (hi - lo + bm - 1) / bm;
+            long incl = t;
+#pragma unroll
+            for (int s = 1; s < 64; s <<= 1) {
+                const long o = shfl_long(incl, lane - s);
+                if (lane >= s) incl += o;
+            }
+            excl = before + incl - t;
+            mine = tile >= excl && tile < before + incl;
+            before += shfl_long(incl, 63);
+        } else {
+            mine = tile >= lo && tile < hi;
+        }
+        const unsigned long long hit = __ballot(mine && g < groups);
+        if (hit && found.g < 0) {
+            const int src = __ffsll((long long)hit) - 1;
+            found.g = base + src;
+            const long rlo = shfl_long(lo, src), rhi = shfl_long(hi, src);
+            const long t0 = bm ? rlo + (tile - shfl_long(excl, src)) * bm : rlo;
+            found.lo = t0;
+            found.hi = bm && t0 + bm < rhi ? t0 + bm : rhi;
+            if (!last) break;
+        }
+        carry = shfl_long(hi, 63);
+    }
+    if (last) *last = uniform_long(carry);
+    found.g = __builtin_amdgcn_readfirstlane(found.g);
+    found.lo = uniform_long(found.lo);
+    found.hi = uniform_long(found.hi);
+    return found;
+}
+
+// Rows [lo, hi) of one run by its number (the same ordered offsets).
+__device__ __forceinline__ Run run_rows(const int64_t* offsets, long rows, int g)
+{
+    const int lane = threadIdx.x & 63;
+    auto bounded = [&](long v) { return v < 0 ? 0 : (v > rows ? rows : v); };
+    long top = 0;                                      // largest of offsets[0 .. g]
+    for (int i = lane; i <= g; i += 64) {
+        const long v = bounded(offsets[i]);
+        top = v > top ? v : top;
+    }
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) {
+        const long o = shfl_long(top, lane ^ s);
+        top = o > top ? o : top;
+    }
+    const long hi = bounded(offsets[g + 1]);
+    Run r = {g, uniform_long(top), 0};
+    r.hi = uniform_long(hi > top ? hi : top);
+    return r;
+}
+
+// Rows of no run become 0 (one workgroup per column block, of any size).
+template <class T>
+__device__ __forceinline__ void fill_rest_rows(const ProductDesc& p, int n0, int n1)
+{
+    long first, last;
+    find_run(p.offsets, p.groups, p.m, -1, 1, &first, &last);
+    const long outside = first + (p.m - last);
+    const long w = n1 - n0;
+    for (long e = threadIdx.x; e < outside * w; e += blockDim.x) {
+        const long q = e / w, j = n0 + e % w;
+        const long i = q < first ? q : last + (q - first);
+        static_cast<T*>(p.epi.C)[i * p.epi.sc_m + j * p.epi.sc_n] = T(0);
+        if (p.epi.pre) static_cast<T*>(p.epi.pre)[i * p.epi.sp_m + j * p.epi.sp_n] = T(0);
+    }
+}
+
+template <class T> struct Mfma;
+template <> struct Mfma<double> {
+    typedef double acc_t __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ acc_t run(double a, double b, acc_t c)
+    {
+        return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0);
+    }
+    // row of register r in a lane (column = lane & 15)
+    static __device__ __forceinline__ int row(int lane, int r) { return (lane >> 4) + 4 * r; }
+};
+template <> struct Mfma<float> {
+    typedef float acc_t __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ acc_t run(float a, float b, acc_t c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ int row(int lane, int r) { return 4 * (lane >> 4) + r; }
+};
+
+// Launchers, one translation unit per type (product_f64.hip, product_f32.hip).  tw: 4 = tiles of
+// 128 x 128, 2 = 64 x 64; mt: 1, 2 or 4 times 16 rows.
+template <class T> int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st);
+template <class T> int launch_product_rows(const ProductDesc& p, int mode, int mt, hipStream_t st);
+
+}  // namespace locus

@@ -1,0 +1,7 @@
+// The float32 instantiations of the fused and grouped products.
+#include "product_rows.h"
+#include "product_tile.h"
+namespace locus {
+template int launch_product_tile<float>(const ProductDesc&, int, int, hipStream_t);
+template int launch_product_rows<float>(const ProductDesc&, int, int, hipStream_t);
+}  // namespace locus

@@ -1,0 +1,307 @@
+"""Fused and grouped matrix products on the matrix cores, with their gradients (torch tensors in, torch
+tensors out; locus_hip_product_* of include/locus_hip.h).  No counterpart in the reference.
+
+    Z = alpha A B + bias,    C = act(Z) + beta residual
+
+  dense_product          one A (m x k), one B (k x n)
+  grouped_product        consecutive runs of A's rows, run g with B[g] and bias[g]: samples that go to
+                         the effects of their own fit (fold, cohort, tissue)
+  dense_product_grad,
+  grouped_product_grad   dA, dB and the bias's gradient from dC and the Z kept by the forward call
+
+`act` is "identity", "logistic" 1 / (1 + e^-z), "probit" Phi(z) (the links of locus()), "softplus"
+log(1 + e^z), "gelu" z Phi(z) or "silu" z / (1 + e^-z).  float64 (the package's type) or float32;
+sums are in that type and in a fixed order, so a call gives the same bits every time.  Any strides; one
+contiguous index per matrix is fast.  The calls are queued on the current stream of the tensors' device
+and return without waiting; outputs and workspaces come from torch's allocator, so the calls can be
+captured into a HIP graph.  They are outside autograd: gradients are the explicit calls here.
+
+`offsets` (groups + 1 int64) and `gather` (int64) stay on the GPU and are not read by the host.  Whatever
+they hold, nothing out of bounds is touched: an offset counts as the largest of 0 and those before it, at
+most the number of rows; a row gathered from outside A comes out NaN.
+"""
+import struct
+
+import torch
+
+from . import _lib
+
+ACTS = {"identity": 0, "logistic": 1, "probit": 2, "softplus": 3, "gelu": 4, "silu": 5}
+_DTYPES = {torch.float64: 0, torch.float32: 1}
+_DENSE, _ROWS, _SUM = 0, 1, 2
+_ARGS = struct.Struct("=3q6i2d27q")              # struct locus_hip_product_args
+_SLOPE_ARGS = struct.Struct("=2q2i13q")          # struct locus_hip_product_slope_args
+
+
+def _fail(msg):
+    raise ValueError(msg)
+
+
+def _check(name, t, like, shape):
+    if not isinstance(t, torch.Tensor):
+        _fail(f"{name} must be a tensor")
+    if t.dtype != like.dtype or t.device != like.device:
+        _fail(f"{name} must be a {like.dtype} tensor on {like.device}, not {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape:
+        _fail(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+
+
+def _operand(name, t, dims):
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        _fail(f"{name} must be a {dims}-dimensional tensor")
+    if t.dtype not in _DTYPES:
+        _fail(f"{name}: float64 or float32, not {t.dtype}")
+    if t.device.type != "cuda":
+        _fail(f"{name} must be on the GPU (no CPU fallback)")
+
+
+def _act(act):
+    try:
+        return ACTS[act]
+    except (KeyError, TypeError):
+        _fail(f"act must be one of {', '.join(ACTS)}, not {act!r}")
+
+
+def _span(t):
+    """First and last byte of a tensor's elements."""
+    lo = t.data_ptr()
+    return lo, lo + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _apart(name, t, others):
+    """An output holds every element once and shares no memory with what the call reads."""
+    if t.numel() == 0:
+        return
+    reach = 1                                    # sizes by growing stride must not fold onto each other
+    for s, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1:
+            if s < reach:
+                _fail(f"{name} has elements that share memory")
+            reach = s * (n - 1) + reach
+    lo, hi = _span(t)
+    for what, o in others:
+        if o is not None and o.numel() and o.element_size():
+            a, b = _span(o)
+            if a < hi and lo < b:
+                _fail(f"{name} shares memory with {what}")
+
+
+def _bias_strides(bias, like, m, n):
+    """(stride over rows, stride over columns) of a bias per column (n,) / (1, n), per row (m, 1), one
+    for all (1, 1) or a whole matrix (m, n)."""
+    if not isinstance(bias, torch.Tensor):
+        _fail("bias must be a tensor")
+    if bias.dtype != like.dtype or bias.device != like.device:
+        _fail(f"bias must be a {like.dtype} tensor on {like.device}")
+    shape = tuple(bias.shape)
+    if len(shape) == 1:
+        if shape[0] != n:
+            _fail(f"bias must have {n} entries, not {shape[0]}")
+        return 0, bias.stride(0)
+    if len(shape) != 2 or shape[0] not in (1, m) or shape[1] not in (1, n):
+        _fail(f"bias must have shape ({n},), ({m}, 1) or ({m}, {n}), not {shape}")
+    return (bias.stride(0) if shape[0] > 1 else 0), (bias.stride(1) if shape[1] > 1 else 0)
+
+
+def _index(name, t, like, size):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.device != like.device or t.dim() != 1:
+        _fail(f"{name} must be a one-dimensional int64 tensor on {like.device}")
+    if size is not None and t.shape[0] != size:
+        _fail(f"{name} must have {size} entries, not {t.shape[0]}")
+    if t.shape[0] > 1 and t.stride(0) != 1:
+        _fail(f"{name} must be contiguous")
+
+
+def _run(dev, fields, like):
+    """fields: of locus_hip_product_args up to the workspace."""
+    lib = _lib.lib()
+    need = lib.locus_hip_product_workspace_bytes(_ARGS.pack(*fields, 0, 0))
+    if need < 0:
+        _lib.check(int(need))
+    ws = 0
+    if need:
+        buf = torch.empty(need, dtype=torch.uint8, device=like.device)
+        ws = buf.data_ptr()
+    args = _ARGS.pack(*fields, ws, need)
+    if dev == torch.cuda.current_device():
+        _lib.check(lib.locus_hip_product_dev(args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(lib.locus_hip_product_dev(args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _strides(t):
+    return t.stride() if t is not None else (0, 0)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else 0
+
+
+def _outputs(A, m, n, out, pre, residual, reads):
+    """Checks or makes C; returns it."""
+    if residual is not None:
+        _check("residual", residual, A, (m, n))
+    if out is None:
+        out = torch.empty((m, n), dtype=A.dtype, device=A.device)
+    else:
+        _check("out", out, A, (m, n))
+        same = residual is not None and out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()
+        _apart("out", out, reads + ([] if same else [("residual", residual)]))
+    if pre is not None:
+        _check("pre", pre, A, (m, n))
+        _apart("pre", pre, reads + [("residual", residual), ("out", out)])
+    return out
+
+
+def dense_product(A, B, bias=None, act="identity", residual=None, alpha=1.0, beta=1.0, out=None, pre=None,
+                  cfg=(0, 0)):
+    """C = act(alpha A B + bias) + beta residual, m x n.
+
+    A (m x k), B (k x n).  bias: (n,) per column, (m, 1) per row or (m, n).  residual: (m, n); `out` may
+    be the residual itself (the same memory and strides), and shares no memory with anything else.
+    pre (m x n), when given, receives Z = alpha A B + bias, which dense_product_grad asks for.  cfg: the
+    kernel's geometry (see include/locus_hip.h), (0, 0) = automatic."""
+    _operand("A", A, 2)
+    _operand("B", B, 2)
+    m, k = A.shape
+    n = B.shape[1]
+    _check("B", B, A, (k, n))
+    code = _act(act)
+    sbias = _bias_strides(bias, A, m, n) if bias is not None else (0, 0)
+    out = _outputs(A, m, n, out, pre, residual, [("A", A), ("B", B), ("bias", bias)])
+    if m and n:
+        _run(A.device.index, (m, n, k, _DTYPES[A.dtype], code, _DENSE, 0, *cfg, alpha, beta,
+                              A.data_ptr(), *A.stride(), B.data_ptr(), *B.stride(), _ptr(bias), *sbias,
+                              _ptr(residual), *_strides(residual), out.data_ptr(), *out.stride(),
+                              _ptr(pre), *_strides(pre), 0, 0, 0, 0, 0, 0, 0), A)
+    return out
+
+
+def grouped_product(A, B, offsets, bias=None, act="identity", residual=None, alpha=1.0, beta=1.0, gather=None,
+                    out=None, pre=None, cfg=(0, 0)):
+    """C[r] = act(alpha A[src(r)] B[g] + bias[g]) + beta residual[r] for the rows r of run g,
+    offsets[g] <= r < offsets[g + 1]; src(r) = gather[r], or r without gather.
+
+    B (groups x k x n), bias (groups x n).  C has as many rows as `gather`, else as A; they are in the order of
+    the runs (gathered rows are not moved back).  Runs may be empty.  Rows of no run are 0 in an `out` that
+    is made here, and are left as they were in one that is given (and in its `pre`)."""
+    _operand("A", A, 2)
+    _operand("B", B, 3)
+    k = A.shape[1]
+    groups, _, n = B.shape
+    _check("B", B, A, (groups, k, n))
+    _index("offsets", offsets, A, groups + 1)
+    m = A.shape[0]
+    if gather is not None:
+        _index("gather", gather, A, None)
+        m = gather.shape[0]
+    if groups < 1:
+        _fail("B must hold at least one group")
+    code = _act(act)
+    if bias is not None:
+        _check("bias", bias, A, (groups, n))
+    fill = out is None
+    out = _outputs(A, m, n, out, pre, residual, [("A", A), ("B", B), ("bias", bias), ("offsets", offsets),
+                                                 ("gather", gather)])
+    if m and n:
+        sb = B.stride()
+        sbias = bias.stride() if bias is not None else (0, 0)
+        _run(A.device.index, (m, n, k, _DTYPES[A.dtype], code, _ROWS, int(fill), *cfg, alpha, beta,
+                              A.data_ptr(), *A.stride(), B.data_ptr(), sb[1], sb[2], _ptr(bias), 0, sbias[1],
+                              _ptr(residual), *_strides(residual), out.data_ptr(), *out.stride(),
+                              _ptr(pre), *_strides(pre), groups, offsets.data_ptr(), sb[0], sbias[0], 0,
+                              _ptr(gather), A.shape[0]), A)
+    return out
+
+
+def _slope(dC, pre, code, m, n, offsets, groups, col_sums, row_sums):
+    """G = dC act'(pre), with its column / row sums; dC itself for the identity."""
+    dev, dt = dC.device, _DTYPES[dC.dtype]
+    G = torch.empty((m, n), dtype=dC.dtype, device=dev) if code else None
+    if (G is None and col_sums is None and row_sums is None) or n == 0 or (m == 0 and col_sums is None):
+        return dC if G is None else G
+    lib = _lib.lib()
+    fields = (m, n, dt, code, dC.data_ptr(), *dC.stride(), _ptr(pre) if code else 0, *_strides(pre), _ptr(G),
+              _ptr(col_sums), _ptr(row_sums), groups, _ptr(offsets))
+    need = lib.locus_hip_product_slope_workspace_bytes(_SLOPE_ARGS.pack(*fields, 0, 0)) if col_sums is not None else 0
+    if need < 0:
+        _lib.check(int(need))
+    buf = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    args = _SLOPE_ARGS.pack(*fields, _ptr(buf), need)
+    with torch.cuda.device(dev):
+        _lib.check(lib.locus_hip_product_slope_dev(args, torch.cuda.current_stream(dev).cuda_stream))
+    return dC if G is None else G
+
+
+def _grad_inputs(dC, A, act, pre, m, n):
+    code = _act(act)
+    _check("dC", dC, A, (m, n))
+    if code:
+        if pre is None:
+            _fail(f"the gradient of {act!r} needs pre, the Z kept by the forward call")
+        _check("pre", pre, A, (m, n))
+    return code
+
+
+def dense_product_grad(dC, A, B, act="identity", pre=None, alpha=1.0, need_A=True, need_B=True, bias_grad=None):
+    """(dA, dB, dbias) of dense_product from dC (m x n), with None for what is not asked for:
+        G = dC act'(pre),  dA = alpha G B',  dB = alpha A' G,
+    dbias = G summed to the shape of the bias: bias_grad = "column" (n,), "row" (m, 1), "matrix" (m, n) or
+    None.  pre is what the forward call stored; the identity needs none.  The residual's gradient is
+    beta dC."""
+    _operand("A", A, 2)
+    _operand("B", B, 2)
+    m, k = A.shape
+    n = B.shape[1]
+    _check("B", B, A, (k, n))
+    code = _grad_inputs(dC, A, act, pre, m, n)
+    if bias_grad not in (None, "column", "row", "matrix"):
+        _fail(f"bias_grad must be None, 'column', 'row' or 'matrix', not {bias_grad!r}")
+    db = None
+    if bias_grad == "column":
+        db = torch.empty(n, dtype=A.dtype, device=A.device)
+    elif bias_grad == "row":
+        db = torch.zeros((m, 1), dtype=A.dtype, device=A.device) if n == 0 else \
+            torch.empty((m, 1), dtype=A.dtype, device=A.device)
+    G = _slope(dC, pre, code, m, n, None, 0, db if bias_grad == "column" else None,
+               db if bias_grad == "row" else None)
+    if bias_grad == "matrix":
+        db = G.clone() if G is dC else G
+    dA = dense_product(G, B.t(), alpha=alpha) if need_A else None
+    dB = dense_product(A.t(), G, alpha=alpha) if need_B else None
+    return dA, dB, db
+
+
+def grouped_product_grad(dC, A, B, offsets, act="identity", pre=None, alpha=1.0, gather=None, need_A=True,
+                         need_B=True, need_bias=False):
+    """(dA, dB, dbias) of grouped_product, with None for what is not asked for:
+        G[r] = dC[r] act'(pre[r]),  dA[r] = alpha G[r] B[g]',
+        dB[g] = alpha sum_{r in g} A[src(r)]' G[r],  dbias[g] = sum_{r in g} G[r].
+    dA has a row for each row of dC: with `gather` it is in the order of the runs, and the gradient of A's
+    row i is the sum of the dA[r] with gather[r] = i.  Rows of no run: 0 in dA.  Empty runs: 0 in dB."""
+    _operand("A", A, 2)
+    _operand("B", B, 3)
+    k = A.shape[1]
+    groups, _, n = B.shape
+    _check("B", B, A, (groups, k, n))
+    _index("offsets", offsets, A, groups + 1)
+    m = A.shape[0]
+    if gather is not None:
+        _index("gather", gather, A, None)
+        m = gather.shape[0]
+    if groups < 1:
+        _fail("B must hold at least one group")
+    code = _grad_inputs(dC, A, act, pre, m, n)
+    db = torch.empty((groups, n), dtype=A.dtype, device=A.device) if need_bias else None
+    G = _slope(dC, pre, code, m, n, offsets, groups, db, None)
+    dA = grouped_product(G, B.transpose(1, 2), offsets, alpha=alpha) if need_A else None
+    dB = None
+    if need_B:
+        dB = torch.empty((groups, k, n), dtype=A.dtype, device=A.device)
+        if k and n:
+            _run(A.device.index, (k, n, m, _DTYPES[A.dtype], 0, _SUM, 0, 0, 0, alpha, 1.0,
+                                  A.data_ptr(), A.stride(1), A.stride(0), G.data_ptr(), *G.stride(), 0, 0, 0, 0, 0, 0,
+                                  dB.data_ptr(), n, 1, 0, 0, 0, groups, offsets.data_ptr(), 0, 0, k * n,
+                                  _ptr(gather), A.shape[0]), A)
+    return dA, dB, db
