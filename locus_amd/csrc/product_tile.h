@@ -28,7 +28,7 @@
 namespace locus {
 
 template <class T, int TW, int BK> struct TileGeom {
-    static constexpr int BM = 32 * TW, BN = 32 * TW, LD = BM + 17;
+    static constexpr int BM = 32 * TW, BN = 32 * TW, LD = BM + 15;
     static constexpr int NQ = BM * BK / 256;
     static constexpr int BUF = BK * LD;                       // one operand, one buffer
     static constexpr int ELEMS = 4 * BUF;
@@ -36,105 +36,244 @@ template <class T, int TW, int BK> struct TileGeom {
 };
 
 template <class T>
-__device__ __forceinline__ T buffer_elem(const char* base, unsigned off)
+__device__ __forceinline__ T buffer_elem(const char* base, unsigned off, unsigned soff)
 {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<char*>(base), 0, 0x7fffffff, 0x00020000 /* 32-bit data format, gfx9 */);
     if constexpr (sizeof(T) == 8)
-        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 0));
     else
-        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0));
 }
 
-template <class T, int TW, int BK, int MODE, bool OFF32>
-__global__ void __launch_bounds__(256, TW == 4 ? 2 : 3) product_tile_kernel(const ProductDesc p)
+// A block of HM x BN sums in LDS (row stride EL) to where it belongs, by 256 threads: VE = 16 bytes of
+// elements along C's contiguous index per thread and turn, addresses stepped, not multiplied out (a
+// 64-bit product per element and matrix made short sums cost 26 us where writing C takes 8).  Partial
+// products and act = identity go U turns at a time, their residuals loaded first; the other functions
+// take long enough to hide one load.
+template <class T, int HM, int BN, int EL>
+__device__ __forceinline__ void store_block(const ProductDesc& p, const T* lds, bool mfast, long m0, int n0,
+                                            int rows, int cols, long bias0, long c0, unsigned bz, bool gr,
+                                            bool outside)
+{
+    constexpr int VE = 16 / (int)sizeof(T), TURNS = HM * BN / VE / 256, U = TURNS < 4 ? TURNS : 4;
+    typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    const int fg = (mfast ? HM : BN) / VE, sp = 256 / fg;  // threads along the fast index, slow ones per turn
+    const int f0 = (int)threadIdx.x % fg * VE, s0 = (int)threadIdx.x / fg;
+    const int cnt = (mfast ? rows : cols) - f0;            // elements of this thread's group that are there
+    const int sEnd = mfast ? cols : rows;
+    if (cnt <= 0 || s0 >= sEnd) return;
+    const bool whole = cnt >= VE;
+    const ProductEpi& e = p.epi;
+    const bool raw = p.part != nullptr;
+    const int act = raw ? LOCUS_HIP_ACT_IDENTITY : e.act;
+    const bool has_res = !raw && e.res, has_pre = !raw && e.pre, has_bias = !raw && e.bias;
+    const long gi = m0 + (mfast ? f0 : s0), gj = n0 + (mfast ? s0 : f0);
+    auto walk = [&](const void* base, long off, long sm, long sn) {
+        return static_cast<T*>(const_cast<void*>(base)) + off + gi * sm + gj * sn;
+    };
+    const long c_m = raw ? p.part_m : e.sc_m, c_n = raw ? p.part_n : e.sc_n;
+    T* c = walk(raw ? p.part : e.C, raw ? bz * p.part_z : c0, c_m, c_n);
+    const long c_f = mfast ? c_m : c_n, c_s = sp * (mfast ? c_n : c_m);
+    const T* res = walk(e.res, 0, e.sr_m, e.sr_n);
+    const long r_f = mfast ? e.sr_m : e.sr_n, r_s = sp * (mfast ? e.sr_n : e.sr_m);
+    const T* bias = walk(e.bias, bias0, e.sb_m, e.sb_n);
+    const long b_f = mfast ? e.sb_m : e.sb_n, b_s = sp * (mfast ? e.sb_n : e.sb_m);
+    T* pre = walk(e.pre, 0, e.sp_m, e.sp_n);
+    const long p_f = mfast ? e.sp_m : e.sp_n, p_s = sp * (mfast ? e.sp_n : e.sp_m);
+    auto get = [&](const T* at, long fs, T* x) {
+        if (whole && fs == 1) {
+            const vec_t v = *reinterpret_cast<const vec_t*>(at);
+#pragma unroll
+            for (int q = 0; q < VE; ++q) x[q] = v[q];
+        } else {
+#pragma unroll
+            for (int q = 0; q < VE; ++q) x[q] = q < cnt ? at[q * fs] : T(0);
+        }
+    };
+    auto put = [&](T* at, long fs, const T* x) {
+        if (whole && fs == 1) {
+            vec_t v;
+#pragma unroll
+            for (int q = 0; q < VE; ++q) v[q] = x[q];
+            *reinterpret_cast<vec_t*>(at) = v;
+        } else {
+#pragma unroll
+            for (int q = 0; q < VE; ++q)
+                if (q < cnt) at[q * fs] = x[q];
+        }
+    };
+    const T* at = lds + (mfast ? f0 * EL + s0 : s0 * EL + f0);
+    const int l_f = mfast ? EL : 1, l_s = mfast ? sp : sp * EL;
+    auto sum = [&](int t, T* x) {
+#pragma unroll
+        for (int q = 0; q < VE; ++q) x[q] = outside ? T(__builtin_nan("")) : at[t * l_s + q * l_f];
+        if (gr && p.k > 0) {
+#pragma unroll
+            for (int q = 0; q < VE; ++q)
+                if (q < cnt) {
+                    const long row = p.gather[gi + (mfast ? q : t * sp)];
+                    if (row < 0 || row >= p.a_rows) x[q] = T(__builtin_nan(""));
+                }
+        }
+    };
+    const T alpha = raw ? T(1) : T(e.alpha), beta = T(e.beta);
+    T b[VE];
+#pragma unroll
+    for (int q = 0; q < VE; ++q) b[q] = T(0);
+    if (has_bias) get(bias, b_f, b);
+    const bool bias_each = has_bias && b_s != 0;           // else: one bias for all turns
+    const int turns = (sEnd - s0 + sp - 1) / sp;           // of this thread, at most TURNS
+    if (act == LOCUS_HIP_ACT_IDENTITY) {
+#pragma unroll 1
+        for (int t0 = 0; t0 < turns; t0 += U) {
+            T r[U][VE];
+            if (has_res) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (t0 + u < turns) get(res + (t0 + u) * r_s, r_f, r[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int t = t0 + u;
+                if (t >= turns) break;
+                T x[VE];
+                sum(t, x);
+                if (bias_each) get(bias + t * b_s, b_f, b);
+#pragma unroll
+                for (int q = 0; q < VE; ++q) x[q] = alpha * x[q] + b[q];
+                if (has_pre) put(pre + t * p_s, p_f, x);
+                if (has_res)
+#pragma unroll
+                    for (int q = 0; q < VE; ++q) x[q] += beta * r[u][q];
+                put(c + t * c_s, c_f, x);
+            }
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int t = 0; t < turns; ++t) {
+        T x[VE], r[VE];
+        if (has_res) get(res + t * r_s, r_f, r);
+        sum(t, x);
+        if (bias_each) get(bias + t * b_s, b_f, b);
+#pragma unroll
+        for (int q = 0; q < VE; ++q) x[q] = alpha * x[q] + b[q];
+        if (has_pre) put(pre + t * p_s, p_f, x);
+#pragma unroll
+        for (int q = 0; q < VE; ++q) x[q] = act_value<T>(act, x[q]);
+        if (has_res)
+#pragma unroll
+            for (int q = 0; q < VE; ++q) x[q] += beta * r[q];
+        put(c + t * c_s, c_f, x);
+    }
+}
+
+// How a kernel is compiled for the operands: FAST with each operand's contiguous index (k or not),
+// or the general form: run-time layouts and 64-bit lane addresses.
+enum { LAY_ANY = 0, LAY_FAST = 1, LAY_A_K = 2, LAY_B_K = 4 };
+
+template <class T, int TW, int BK, int PF, int MODE, int LAY>
+__global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(const ProductDesc p)
 {
     typedef TileGeom<T, TW, BK> G;
     typedef typename Mfma<T>::acc_t acc_t;
     constexpr int BM = G::BM, BN = G::BN, LD = G::LD, NQ = G::NQ, BUF = G::BUF;
+    constexpr bool FAST = LAY & LAY_FAST, AKF = LAY & LAY_A_K, BKF = LAY & LAY_B_K;
     __shared__ T lds[G::ELEMS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave >> 1, wn = wave & 1;
 
-    // which tile
-    int n0 = blockIdx.y * BN, nEnd = p.n;
+    // Which tile.  Workgroups go to the 8 XCDs in turn by their number; each XCD takes a contiguous
+    // eighth of the list below, in which 64 neighbours (what an XCD holds at once) are 8 x 8 tiles of
+    // one slice of k, so that strips of A and B are read from its L2 by the others.
+    unsigned bx, by, bz;
+    {
+        const unsigned gx = gridDim.x, gy = gridDim.y, each = gx * gy, total = each * gridDim.z;
+        const unsigned lin = blockIdx.x + gx * (blockIdx.y + gy * blockIdx.z);
+        const unsigned xcd = lin & 7, rem = total & 7;
+        const unsigned w = xcd * (total >> 3) + (xcd < rem ? xcd : rem) + (lin >> 3);
+        bz = w / each;
+        const unsigned t = w - bz * each;
+        const unsigned panel = t / (8 * gy), r = t - panel * 8 * gy;
+        const unsigned high = gx - panel * 8 < 8 ? gx - panel * 8 : 8;
+        by = r / high;
+        bx = panel * 8 + r - by * high;
+    }
+    const int n0 = by * BN, nEnd = p.n;
     long m0, mEnd;                      // rows of C
-    long kb = 0, kEnd = p.k;
+    int kb = 0, kEnd = p.k;
     const T* A = static_cast<const T*>(p.A);
     const T* B = static_cast<const T*>(p.B);
     long bias0 = 0, c0 = 0;
-    int z = 0;
     if constexpr (MODE == PRODUCT_DENSE) {
-        m0 = (long)blockIdx.x * BM;
+        m0 = (long)bx * BM;
         mEnd = p.m;
     } else if constexpr (MODE == PRODUCT_ROWS) {
-        if (p.fill_rest && blockIdx.x == gridDim.x - 1) {
-            if (blockIdx.z == 0) fill_rest_rows<T>(p, n0, n0 + BN < p.n ? n0 + BN : p.n);
+        if (p.fill_rest && bx == gridDim.x - 1) {
+            if (bz == 0) fill_rest_rows<T>(p, n0, n0 + BN < p.n ? n0 + BN : p.n);
             return;
         }
-        const Run r = find_run(p.offsets, p.groups, p.m, blockIdx.x, BM);
+        const Run r = find_run(p.offsets, p.groups, p.m, bx, BM);
         if (r.g < 0) return;
         m0 = r.lo;
         mEnd = r.hi;
         B += r.g * p.sb_g;
         bias0 = r.g * p.sbias_g;
     } else {
-        const Run r = run_rows(p.offsets, p.k, blockIdx.z);
-        m0 = (long)blockIdx.x * BM;
+        const Run r = run_rows(p.offsets, p.k, bz);
+        m0 = (long)bx * BM;
         mEnd = p.m;
-        kb = r.lo;
-        kEnd = r.hi;
+        kb = (int)r.lo;
+        kEnd = (int)r.hi;
         c0 = r.g * p.sc_g;
     }
     if constexpr (MODE != PRODUCT_SUM) {
         if (p.part) {
-            z = blockIdx.z;
-            kb = (long)z * p.kchunk;
+            kb = bz * p.kchunk;
             kEnd = kb + p.kchunk < p.k ? kb + p.kchunk : p.k;
         }
     }
 
-    // element -> (row, k) follows the contiguous index of each operand; gathered k rows are taken
-    // one per wave at a time (row index on the scalar unit)
-    const bool gk = MODE == PRODUCT_SUM && p.gather != nullptr;
-    const bool a_kfast = p.sa_k == 1 && !gk;
-    const bool b_kfast = p.sb_k == 1;
-    const long mRows = mEnd - m0;
-    typedef typename std::conditional<OFF32, unsigned, long>::type off_t;
-    off_t oa[NQ], ob[NQ];
-    int ak[NQ], bk[NQ];
-    T* al[NQ];
-    T* bl[NQ];
-    bool bad[NQ];                       // gathered rows outside A (MODE ROWS)
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const int e = tid + q * 256;
-        int am;
-        if (a_kfast) { ak[q] = e % BK; am = e / BK; } else { am = e % BM; ak[q] = e / BM; }
-        al[q] = lds + ak[q] * LD + am;
-        const long i = am < mRows ? am : 0;
-        long row = i;
-        bad[q] = false;
-        if constexpr (MODE == PRODUCT_ROWS && !OFF32) {
-            row = m0 + i;
-            if (p.gather) {
-                row = p.gather[row];
-                bad[q] = row < 0 || row >= p.a_rows;
-                if (bad[q]) row = 0;
-            }
-        }
-        oa[q] = (off_t)((row * p.sa_m + (gk ? 0 : ak[q] * p.sa_k)) * (long)sizeof(T));
-        int bn;
-        if (b_kfast) { bk[q] = e % BK; bn = e / BK; } else { bn = e % BN; bk[q] = e / BN; }
-        bl[q] = lds + 2 * BUF + bk[q] * LD + bn;
-        const long j = n0 + bn < nEnd ? bn : 0;
-        ob[q] = (off_t)((j * p.sb_n + bk[q] * p.sb_k) * (long)sizeof(T));
-    }
-    const bool rows64 = MODE == PRODUCT_ROWS && !OFF32;
-    const char* Ab = reinterpret_cast<const char*>(A + (rows64 ? 0 : m0 * p.sa_m) + (gk ? 0 : kb * p.sa_k));
+    // Element q of a thread: k-fast operands (k contiguous) k = tid % BK, row = tid / BK + q 256 / BK;
+    // else row = tid % BM, k = tid / BM + q 256 / BM (the same k for a whole wave).
+    constexpr int QK = 256 / BK, QM = 256 / BM;
+    constexpr int sz = (int)sizeof(T);
+    const bool akf = FAST ? AKF : (p.sa_k == 1 && !(MODE == PRODUCT_SUM && p.gather));
+    const bool bkf = FAST ? BKF : p.sb_k == 1;
+    const int ak0 = akf ? tid % BK : __builtin_amdgcn_readfirstlane(tid / BM);
+    const int bk0 = bkf ? tid % BK : __builtin_amdgcn_readfirstlane(tid / BM);
+    const int mRows = (int)(mEnd - m0 < BM ? mEnd - m0 : BM), nCols = nEnd - n0 < BN ? nEnd - n0 : BN;
+    T* const al = lds + (akf ? (tid % BK) * LD + tid / BK : (tid / BM) * LD + tid % BM);
+    T* const bl = lds + 2 * BUF + (bkf ? (tid % BK) * LD + tid / BK : (tid / BM) * LD + tid % BM);
+    const int aq = akf ? QK : QM * LD, bq = bkf ? QK : QM * LD;      // LDS step of q
+
+    // Row of A behind row i of the tile; gathered indexes outside A count as 0 here (they never reach
+    // a result: the epilogue makes it NaN).  Base: the tile's first row, gathered: A's first.
+    const bool gr = MODE == PRODUCT_ROWS && p.gather, gs = MODE == PRODUCT_SUM && p.gather;
+    auto in_a = [&](long row) { return row >= 0 && row < p.a_rows ? row : 0; };
+    auto a_row = [&](int i) -> long {
+        const int c = i < mRows ? i : 0;
+        return gr ? in_a(p.gather[m0 + c]) : c;
+    };
+    const char* Ab = reinterpret_cast<const char*>(A + (gr ? 0 : m0 * p.sa_m) + (gs ? 0 : kb * p.sa_k));
     const char* Bb = reinterpret_cast<const char*>(B + (long)n0 * p.sb_n + kb * p.sb_k);
-    const long da = (gk ? 0 : BK * p.sa_k) * (long)sizeof(T), db = BK * p.sb_k * (long)sizeof(T);
+    const long da = (gs ? 0 : BK * p.sa_k) * sz, db = BK * p.sb_k * sz;
+    // Lane offsets in bytes: one per element where k is contiguous (rows are clamped one by one), else one, and
+    // the step of q on the scalar unit.
+    typedef typename std::conditional<FAST, unsigned, long>::type off_t;
+    constexpr int NA = FAST && !AKF ? 1 : NQ, NB = FAST && !BKF ? 1 : NQ;
+    off_t oa[NA], ob[NB];
+#pragma unroll
+    for (int q = 0; q < NA; ++q)
+        oa[q] = (off_t)((akf ? a_row(tid / BK + q * QK) * p.sa_m + ak0 * p.sa_k
+                             : a_row(tid % BM) * p.sa_m + (gs ? 0 : (ak0 + q * QM) * p.sa_k)) * sz);
+#pragma unroll
+    for (int q = 0; q < NB; ++q) {
+        const int j = bkf ? tid / BK + q * QK : tid % BM;
+        ob[q] = (off_t)(((j < nCols ? j : 0) * p.sb_n + (bkf ? bk0 : bk0 + q * QM) * p.sb_k) * sz);
+    }
 
     acc_t acc[TW][TW];
 #pragma unroll
@@ -142,111 +281,164 @@ __global__ void __launch_bounds__(256, TW == 4 ? 2 : 3) product_tile_kernel(cons
 #pragma unroll
         for (int j = 0; j < TW; ++j) acc[i][j] = (acc_t){0, 0, 0, 0};
 
-    const T qnan = T(__builtin_nan(""));
-    auto get = [&](const char* base, off_t off) -> T {
-        if constexpr (OFF32) return buffer_elem<T>(base, off);
-        else return *reinterpret_cast<const T*>(base + off);
+    const int tiles = kEnd > kb ? (kEnd - kb + BK - 1) / BK : 0;   // K-tiles
+    T ra[PF][NQ], rb[PF][NQ];           // [stage]: K-tiles on their way
+    // Element q of the K-tile that starts at k0.  Gathered sums: one row of A per wave and element.
+    auto get_a = [&](int q, int k0) -> T {
+        const int k = k0 + ak0 + (akf ? 0 : q * QM);
+        if (MODE == PRODUCT_SUM && gs) {
+            const long row = in_a(p.gather[k]) * p.sa_k * sz;
+            if constexpr (FAST) return buffer_elem<T>(Ab, oa[0], (unsigned)row);
+            else return *reinterpret_cast<const T*>(Ab + row + oa[q]);
+        }
+        if constexpr (FAST) return buffer_elem<T>(Ab, oa[AKF ? q : 0], AKF ? 0u : (unsigned)(q * QM * p.sa_k * sz));
+        else return *reinterpret_cast<const T*>(Ab + oa[q]);
     };
-    T ra[NQ], rb[NQ];
-    auto get_a = [&](int q, long k) -> T {              // k: its place in the sum (gathered sums)
-        if constexpr (MODE == PRODUCT_SUM) {
-            if (gk) {
-                const long row = uniform_long(p.gather[uniform_long(k)]);
-                if (row < 0 || row >= p.a_rows) return qnan;
-                return get(Ab + row * p.sa_k * (long)sizeof(T), oa[q]);
+    auto get_b = [&](int q) -> T {
+        if constexpr (FAST) return buffer_elem<T>(Bb, ob[BKF ? q : 0], BKF ? 0u : (unsigned)(q * QM * p.sb_k * sz));
+        else return *reinterpret_cast<const T*>(Bb + ob[q]);
+    };
+    // The K-tile whose first k is k0, elements [q0, q1) of each operand, to registers (stage st).
+    auto load_part = [&](auto stc, auto wholec, int k0, int q0, int q1) {
+        constexpr int st = decltype(stc)::value % PF;
+        if (decltype(wholec)::value || k0 + BK <= kEnd) {
+#pragma unroll
+            for (int q = q0; q < q1; ++q) {
+                ra[st][q] = get_a(q, k0);
+                rb[st][q] = get_b(q);
             }
-        }
-        if constexpr (MODE == PRODUCT_ROWS && !OFF32) {
-            if (bad[q]) return qnan;
-        }
-        return get(Ab, oa[q]);
-    };
-    auto load_tile = [&](long k0) {
-        if (k0 + BK <= kEnd) {
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) ra[q] = get_a(q, k0 + ak[q]);
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) rb[q] = get(Bb, ob[q]);
         } else {
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) ra[q] = k0 + ak[q] < kEnd ? get_a(q, k0 + ak[q]) : T(0);
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) rb[q] = k0 + bk[q] < kEnd ? get(Bb, ob[q]) : T(0);
+            for (int q = q0; q < q1; ++q) {
+                ra[st][q] = k0 + ak0 + (akf ? 0 : q * QM) < kEnd ? get_a(q, k0) : T(0);
+                rb[st][q] = k0 + bk0 + (bkf ? 0 : q * QM) < kEnd ? get_b(q) : T(0);
+            }
         }
+    };
+    auto advance = [&]() {
         Ab += da;
         Bb += db;
     };
+    auto write_part = [&](auto bufc, int q0, int q1) {
+        constexpr int buf = decltype(bufc)::value, st = buf % PF;
+#pragma unroll
+        for (int q = q0; q < q1; ++q) {
+            al[buf * BUF + q * aq] = ra[st][q];
+            bl[buf * BUF + q * bq] = rb[st][q];
+        }
+    };
     const T* ar = lds + (lane >> 4) * LD + wm * 16 * TW + (lane & 15);
     const T* br = lds + 2 * BUF + (lane >> 4) * LD + wn * 16 * TW + (lane & 15);
-    auto k_tile = [&](auto bufc, long k0) {
+    T fa[2][TW], fb[2][TW];             // operands of this and of the next step
+    auto read_step = [&](auto bufc, auto sc) {
+        constexpr int buf = decltype(bufc)::value, s = decltype(sc)::value;
+#pragma unroll
+        for (int i = 0; i < TW; ++i) fa[s & 1][i] = ar[buf * BUF + 4 * s * LD + i * 16];
+#pragma unroll
+        for (int j = 0; j < TW; ++j) fb[s & 1][j] = br[buf * BUF + 4 * s * LD + j * 16];
+    };
+    constexpr int S = BK / 4;           // steps of a K-tile
+    constexpr int MS = S / 2;           // the first MS of them move the coming K-tiles
+    static_assert(S % 2 == 0 && NQ % MS == 0, "steps and elements");
+    // K-tile t, its step 0 already in fa[0], fb[0].  Every step first reads the operands of the next
+    // one (the last step those of the next K-tile, behind the barrier that publishes it), so that a
+    // wave's matrix instructions never wait for an LDS read just issued; tile t + 1 goes to LDS and
+    // tile t + 1 + PF is requested in pieces between them.  CHECK: the last tiles, which ask what is left.
+    auto k_tile = [&](auto bufc, auto checkc, int t) {
         constexpr int buf = decltype(bufc)::value;
-        if (k0 + BK < kEnd) {
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) al[q][(buf ^ 1) * BUF] = ra[q];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) bl[q][(buf ^ 1) * BUF] = rb[q];
-        }
-        if (k0 + 2 * BK < kEnd) load_tile(k0 + 2 * BK);
-#pragma unroll
-        for (int s = 0; s < BK / 4; ++s) {
-            T a[TW], b[TW];
-#pragma unroll
-            for (int i = 0; i < TW; ++i) a[i] = ar[buf * BUF + 4 * s * LD + i * 16];
-#pragma unroll
-            for (int j = 0; j < TW; ++j) b[j] = br[buf * BUF + 4 * s * LD + j * 16];
+        constexpr bool CHECK = decltype(checkc)::value;
+        constexpr auto nextc = std::integral_constant<int, buf ^ 1>{};
+        const bool more = !CHECK || t + 1 < tiles;
+        const int kl = kb + (t + 1 + PF) * BK;
+        const bool ask = !CHECK || t + 1 + PF < tiles;
+        auto step = [&](auto sc) {
+            constexpr int s = decltype(sc)::value;
+            if constexpr (s + 1 < S) {
+                read_step(bufc, std::integral_constant<int, s + 1>{});
+            } else {
+                __syncthreads();
+                if (more) read_step(nextc, std::integral_constant<int, 0>{});
+            }
+            if constexpr (s < MS) {
+                constexpr int q0 = s * (NQ / MS), q1 = q0 + NQ / MS;
+                if (more) write_part(nextc, q0, q1);
+                if (ask) {
+                    load_part(nextc, std::bool_constant<!CHECK>{}, kl, q0, q1);
+                    if (s == MS - 1) advance();
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < TW; ++i)
 #pragma unroll
-                for (int j = 0; j < TW; ++j) acc[i][j] = Mfma<T>::run(a[i], b[j], acc[i][j]);
+                for (int j = 0; j < TW; ++j) acc[i][j] = Mfma<T>::run(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+        if constexpr (S == 8) {
+            step(std::integral_constant<int, 4>{});
+            step(std::integral_constant<int, 5>{});
+            step(std::integral_constant<int, 6>{});
+            step(std::integral_constant<int, 7>{});
+        }
+    };
+    if (tiles > 0) {
+        constexpr auto b0 = std::integral_constant<int, 0>{};
+        constexpr auto b1 = std::integral_constant<int, 1>{};
+        load_part(b0, std::false_type{}, kb, 0, NQ);
+        advance();
+        if (PF == 2 && tiles > 1) {
+            load_part(b1, std::false_type{}, kb + BK, 0, NQ);
+            advance();
+        }
+        write_part(b0, 0, NQ);
+        if (tiles > PF) {
+            load_part(std::integral_constant<int, PF>{}, std::false_type{}, kb + PF * BK, 0, NQ);
+            advance();
         }
         __syncthreads();
-    };
-    if (kb < kEnd) {
-        load_tile(kb);
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) al[q][0] = ra[q];
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) bl[q][0] = rb[q];
-        if (kb + BK < kEnd) load_tile(kb + BK);
-        __syncthreads();
-        for (long k0 = kb; k0 < kEnd; k0 += 2 * BK) {
-            k_tile(std::integral_constant<int, 0>{}, k0);
-            if (k0 + BK < kEnd) k_tile(std::integral_constant<int, 1>{}, k0 + BK);
+        read_step(b0, b0);
+        const int full = (kEnd - kb) / BK;
+        int t = 0;
+        for (; t + 2 + PF < full; t += 2) {
+            k_tile(b0, std::false_type{}, t);
+            k_tile(b1, std::false_type{}, t + 1);
+        }
+        for (; t < tiles; t += 2) {
+            k_tile(b0, std::true_type{}, t);
+            if (t + 1 < tiles) k_tile(b1, std::true_type{}, t + 1);
         }
     }
 
-    // Through LDS, half the rows at a time.
-    constexpr int HM = BM / 2, EL = BN + 1;
+    // A gathered sum over a row outside A: its run's C is NaN.
+    bool outside = false;
+    if (gs) {
+        for (int k = kb + tid; k < kEnd; k += 256) outside |= p.gather[k] < 0 || p.gather[k] >= p.a_rows;
+        outside = __syncthreads_or(outside);
+    }
+
+    // Through LDS, all rows at a time or half of them, then along C's contiguous index.
+    constexpr int HALVES = BM * (BN + 1) <= G::ELEMS ? 1 : 2, HM = BM / HALVES, EL = BN + 1;
     const bool mfast = p.part ? p.part_m == 1 : (p.epi.sc_n != 1 && p.epi.sc_m == 1);
-    ProductEpi epi = p.epi;
-    epi.C = static_cast<T*>(p.epi.C) + c0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (wm == h) {
+    for (int h = 0; h < HALVES; ++h) {
+        if (HALVES == 1 || wm == h) {
+            T* at = lds + (HALVES == 1 ? wm * 16 * TW * EL : 0) + wn * 16 * TW + (lane & 15);
 #pragma unroll
             for (int i = 0; i < TW; ++i)
 #pragma unroll
                 for (int j = 0; j < TW; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        lds[(i * 16 + Mfma<T>::row(lane, r)) * EL + wn * 16 * TW + j * 16 +
-                            (lane & 15)] = acc[i][j][r];
+                        at[(i * 16 + Mfma<T>::row(lane, r)) * EL + j * 16] = acc[i][j][r];
         }
         __syncthreads();
-#pragma unroll 1
-        for (int e = tid; e < HM * BN; e += 256) {
-            const int i = mfast ? e % HM : e / BN, j = mfast ? e / HM : e % BN;
-            const long gi = m0 + h * HM + i;
-            const int gj = n0 + j;
-            if (gi < mEnd && gj < nEnd) {
-                const T v = lds[i * EL + j];
-                if (p.part)
-                    static_cast<T*>(p.part)[z * p.part_z + gi * p.part_m + gj * p.part_n] = v;
-                else
-                    epi_store<T>(epi, bias0, gi, gj, v);
-            }
-        }
-        __syncthreads();
+        const int rows = (int)(mEnd - m0 - h * HM < HM ? mEnd - m0 - h * HM : HM);
+        store_block<T, HM, BN, EL>(p, lds, mfast, m0 + h * HM, n0, rows, nCols, bias0, c0, bz, gr, outside);
+        if (h + 1 < HALVES) __syncthreads();
     }
 }
 
@@ -254,11 +446,19 @@ template <class T>
 int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
 {
     constexpr int BK = sizeof(T) == 8 ? 16 : 32;
-    const int bm = 32 * tw;
+    int bm = 32 * tw;
+    // 32-bit lane offsets: a K-tile's elements lie within 2^31 bytes behind its first one (a gathered
+    // A: all of A does)
     const long lim = ((1L << 31) - 1) / (long)sizeof(T);
-    const bool off32 = p.gather == nullptr && p.sa_m >= 0 && p.sa_k >= 0 && p.sb_n >= 0 &&
-                       p.sb_k >= 0 && (bm - 1) * p.sa_m + (BK - 1) * p.sa_k <= lim &&
+    const long a_m = mode == PRODUCT_ROWS && p.gather ? p.a_rows : bm, a_k = mode == PRODUCT_SUM && p.gather ? p.a_rows : BK;
+    const bool off32 = p.sa_m >= 0 && p.sa_k >= 0 && p.sb_n >= 0 && p.sb_k >= 0 &&
+                       (a_m - 1) * p.sa_m + (a_k - 1) * p.sa_k <= lim &&
                        (bm - 1) * p.sb_n + (BK - 1) * p.sb_k <= lim;
+    // Compiled fast: every layout of one matrix pair; runs of rows with A contiguous along a row; sums over
+    // runs with both operands contiguous along theirs.  The rest takes the general form (tiles of 64).
+    const bool ak = p.sa_k == 1, bk = p.sb_k == 1;
+    const bool fast = off32 && (mode == PRODUCT_DENSE || (mode == PRODUCT_ROWS ? ak : !bk && (!ak || p.gather)));
+    if (!fast) bm = 64;
     const unsigned gy = (unsigned)((p.n + bm - 1) / bm);
     unsigned gx = (unsigned)((p.m + bm - 1) / bm), gz = p.part ? (unsigned)p.nz : 1u;
     // runs of rows: at most m / bm full tiles and one partial tile per run
@@ -269,17 +469,25 @@ int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
         return 0;
     };
     auto pick = [&](auto twc) {
-        constexpr int TW = decltype(twc)::value;
-        if (mode == PRODUCT_DENSE)
-            return off32 ? go(product_tile_kernel<T, TW, BK, PRODUCT_DENSE, true>)
-                         : go(product_tile_kernel<T, TW, BK, PRODUCT_DENSE, false>);
+        constexpr int TW = decltype(twc)::value, PF = TW == 2 ? 2 : 1;
+        if (mode == PRODUCT_DENSE) {
+            if (ak)
+                return bk ? go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST | LAY_A_K | LAY_B_K>)
+                          : go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST | LAY_A_K>);
+            return bk ? go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST | LAY_B_K>)
+                      : go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST>);
+        }
         if (mode == PRODUCT_ROWS)
-            return off32 ? go(product_tile_kernel<T, TW, BK, PRODUCT_ROWS, true>)
-                         : go(product_tile_kernel<T, TW, BK, PRODUCT_ROWS, false>);
-        return off32 ? go(product_tile_kernel<T, TW, BK, PRODUCT_SUM, true>)
-                     : go(product_tile_kernel<T, TW, BK, PRODUCT_SUM, false>);
+            return bk ? go(product_tile_kernel<T, TW, BK, PF, PRODUCT_ROWS, LAY_FAST | LAY_A_K | LAY_B_K>)
+                      : go(product_tile_kernel<T, TW, BK, PF, PRODUCT_ROWS, LAY_FAST | LAY_A_K>);
+        return go(product_tile_kernel<T, TW, BK, PF, PRODUCT_SUM, LAY_FAST>);
     };
-    const int rc = tw == 4 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 2>{});
+    auto any = [&]() {
+        if (mode == PRODUCT_DENSE) return go(product_tile_kernel<T, 2, BK, 1, PRODUCT_DENSE, LAY_ANY>);
+        if (mode == PRODUCT_ROWS) return go(product_tile_kernel<T, 2, BK, 1, PRODUCT_ROWS, LAY_ANY>);
+        return go(product_tile_kernel<T, 2, BK, 1, PRODUCT_SUM, LAY_ANY>);
+    };
+    const int rc = !fast ? any() : tw == 4 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 2>{});
     if (rc) return rc;
     LOCUS_HIP_CHECK(hipGetLastError());
     return 0;
