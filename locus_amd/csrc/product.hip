@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(256) product_sums_join_kernel(const T* sums, i
     const long e = (long)blockIdx.x * 256 + threadIdx.x;
     if (e >= len) return;
     T v = T(0);
+#pragma unroll 8
     for (int q = 0; q < parts; ++q) v += sums[q * len + e];
     out[e] = v;
 }
@@ -159,7 +160,7 @@ Plan plan_product(const locus_hip_product_args& a)
         const long mt = runs ? (long)(a.groups * ((long)(avg + bm - 1) / bm)) : (a.m + bm - 1) / bm;
         const long tiles = std::max<long>(mt, 1) * ((a.n + bm - 1) / bm);
         for (long nz = 1; nz <= 32; ++nz) {
-            if (a.cfg[1] && nz != a.cfg[1]) continue;
+            if (a.cfg[1]) nz = a.cfg[1];
             const long chunk = ((a.k + nz - 1) / nz + bk - 1) / bk * bk;
             if (!a.cfg[1] && nz > 1 && chunk < 8 * bk) break;
             const long used = a.k > 0 ? (a.k + chunk - 1) / chunk : 1;
@@ -173,6 +174,7 @@ Plan plan_product(const locus_hip_product_args& a)
                 pl.nz = (int)used;
                 pl.kchunk = chunk;
             }
+            if (a.cfg[1]) break;
         }
     }
     if (pl.tw == 0) pl.tw = 4;

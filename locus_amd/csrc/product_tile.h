@@ -283,36 +283,36 @@ __global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(cons
 
     const int tiles = kEnd > kb ? (kEnd - kb + BK - 1) / BK : 0;   // K-tiles
     T ra[PF][NQ], rb[PF][NQ];           // [stage]: K-tiles on their way
-    // Element q of the K-tile that starts at k0.  Gathered sums: one row of A per wave and element.
-    auto get_a = [&](int q, int k0) -> T {
-        const int k = k0 + ak0 + (akf ? 0 : q * QM);
+    // Element q of the K-tile that starts at k0; `in`: k is not beyond the end.  An element beyond it is 0: FAST
+    // asks for an offset outside the buffer resource, which the hardware answers with 0 (no branches in
+    // short sums).  Gathered sums: one row of A per wave and element.
+    auto get_a = [&](int q, int k0, bool in) -> T {
         if (MODE == PRODUCT_SUM && gs) {
-            const long row = in_a(p.gather[k]) * p.sa_k * sz;
-            if constexpr (FAST) return buffer_elem<T>(Ab, oa[0], (unsigned)row);
+            if constexpr (!FAST) if (!in) return T(0);
+            const int k = k0 + ak0 + q * QM;                    // the same for a whole wave
+            const long row = in_a(p.gather[in ? k : kb]) * p.sa_k * sz;
+            if constexpr (FAST) return buffer_elem<T>(Ab, in ? oa[0] : 0x80000000u, (unsigned)row);
             else return *reinterpret_cast<const T*>(Ab + row + oa[q]);
         }
-        if constexpr (FAST) return buffer_elem<T>(Ab, oa[AKF ? q : 0], AKF ? 0u : (unsigned)(q * QM * p.sa_k * sz));
-        else return *reinterpret_cast<const T*>(Ab + oa[q]);
+        if constexpr (FAST)
+            return buffer_elem<T>(Ab, in ? oa[AKF ? q : 0] : 0x80000000u, AKF ? 0u : (unsigned)(q * QM * p.sa_k * sz));
+        else
+            return in ? *reinterpret_cast<const T*>(Ab + oa[q]) : T(0);
     };
-    auto get_b = [&](int q) -> T {
-        if constexpr (FAST) return buffer_elem<T>(Bb, ob[BKF ? q : 0], BKF ? 0u : (unsigned)(q * QM * p.sb_k * sz));
-        else return *reinterpret_cast<const T*>(Bb + ob[q]);
+    auto get_b = [&](int q, bool in) -> T {
+        if constexpr (FAST)
+            return buffer_elem<T>(Bb, in ? ob[BKF ? q : 0] : 0x80000000u, BKF ? 0u : (unsigned)(q * QM * p.sb_k * sz));
+        else
+            return in ? *reinterpret_cast<const T*>(Bb + ob[q]) : T(0);
     };
     // The K-tile whose first k is k0, elements [q0, q1) of each operand, to registers (stage st).
     auto load_part = [&](auto stc, auto wholec, int k0, int q0, int q1) {
         constexpr int st = decltype(stc)::value % PF;
-        if (decltype(wholec)::value || k0 + BK <= kEnd) {
+        constexpr bool whole = decltype(wholec)::value;
 #pragma unroll
-            for (int q = q0; q < q1; ++q) {
-                ra[st][q] = get_a(q, k0);
-                rb[st][q] = get_b(q);
-            }
-        } else {
-#pragma unroll
-            for (int q = q0; q < q1; ++q) {
-                ra[st][q] = k0 + ak0 + (akf ? 0 : q * QM) < kEnd ? get_a(q, k0) : T(0);
-                rb[st][q] = k0 + bk0 + (bkf ? 0 : q * QM) < kEnd ? get_b(q) : T(0);
-            }
+        for (int q = q0; q < q1; ++q) {
+            ra[st][q] = get_a(q, k0, whole || k0 + ak0 + (akf ? 0 : q * QM) < kEnd);
+            rb[st][q] = get_b(q, whole || k0 + bk0 + (bkf ? 0 : q * QM) < kEnd);
         }
     };
     auto advance = [&]() {
@@ -368,10 +368,12 @@ __global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(cons
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
+            if (!CHECK || 4 * s < kEnd - (kb + t * BK)) {       // steps beyond the end have nothing to add
 #pragma unroll
-            for (int i = 0; i < TW; ++i)
+                for (int i = 0; i < TW; ++i)
 #pragma unroll
-                for (int j = 0; j < TW; ++j) acc[i][j] = Mfma<T>::run(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+                    for (int j = 0; j < TW; ++j) acc[i][j] = Mfma<T>::run(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+            }
             __builtin_amdgcn_sched_barrier(0);
         };
         step(std::integral_constant<int, 0>{});
