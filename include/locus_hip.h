@@ -289,12 +289,9 @@ int locus_hip_gemm_dev(int64_t m, int64_t n, int64_t k, double alpha, const doub
  *           its own fit (fold, cohort, tissue).  Runs may be empty; rows before the first and behind
  *           the last run are left as they were (fill_rest: become 0 in C and pre).  gather: row r
  *           reads A's row gather[r] (the same row any number of times); C's rows are not moved.
- *   LOCUS_HIP_PRODUCT_SUM    the runs cut the SUMMED index: C + g sc_g = alpha A_g B_g over the k
- *           in [offsets[g], offsets[g + 1]) (the gradient of the runs' effects; 0 for an empty run).
- *           gather: place r of the sum reads A's elements at place gather[r].  No bias, res, pre.
  * offsets and gather are device arrays, never read by the host.  Whatever they hold, nothing out of
  * bounds is touched: an offset counts as the largest of 0 and those before it, at most the number of
- * rows, and a gathered index outside [0, a_rows) makes its row (in a sum: its run's C) NaN. */
+ * rows, and a gathered index outside [0, a_rows) makes its row NaN (in a gradient: its run's dB). */
 #define LOCUS_HIP_F64 0
 #define LOCUS_HIP_F32 1
 #define LOCUS_HIP_ACT_IDENTITY 0    /* z                                                        */
@@ -305,13 +302,12 @@ int locus_hip_gemm_dev(int64_t m, int64_t n, int64_t k, double alpha, const doub
 #define LOCUS_HIP_ACT_SILU 5        /* z / (1 + exp(-z))                                        */
 #define LOCUS_HIP_PRODUCT_DENSE 0
 #define LOCUS_HIP_PRODUCT_ROWS 1
-#define LOCUS_HIP_PRODUCT_SUM 2
 typedef struct locus_hip_product_args {
     int64_t m, n, k;            /* m, k < 2^30, n <= 4194240                                    */
     int32_t dtype, act, mode, fill_rest;
-    int32_t cfg[2];             /* kernel geometry, 0 = automatic: cfg[0] = 1, 2, 4 (kernel for few
-                                   rows, tiles of 16, 32, 64 rows), 64, 128 (tiles of 64, 128 rows and
-                                   columns); cfg[1] = slices of k (1..256)                       */
+    int32_t cfg[2];             /* kernel geometry, 0 = automatic: cfg[0] = 16 (kernel for few rows),
+                                   64, 128 (tiles of so many rows and columns); cfg[1] = slices of k
+                                   (1..256)                                                     */
     double alpha, beta;
     const void* A; int64_t sa_m, sa_k;
     const void* B; int64_t sb_k, sb_n;
@@ -320,33 +316,38 @@ typedef struct locus_hip_product_args {
     void* C; int64_t sc_m, sc_n;
     void* pre; int64_t sp_m, sp_n;                /* or NULL: receives Z; not C                 */
     int64_t groups; const int64_t* offsets;       /* [groups + 1]                               */
-    int64_t sb_g, sbias_g, sc_g;
-    const int64_t* gather; int64_t a_rows;        /* [m] (SUM: [k]) or NULL                     */
+    int64_t sb_g, sbias_g;
+    const int64_t* gather; int64_t a_rows;        /* [m] or NULL                                */
     void* workspace; int64_t workspace_bytes;
 } locus_hip_product_args;
 int locus_hip_product_dev(const locus_hip_product_args* args, void* stream);
 /* Bytes of workspace for that call (pointers are not looked at), or a negative error. */
 int64_t locus_hip_product_workspace_bytes(const locus_hip_product_args* args);
 
-/* The first step of the gradient: G = dC act'(pre), row-major m x n, with
- *   col_sums[max(groups, 1)][n] = its sums over the rows of each run (gradient of a bias per column),
- *   row_sums[m] = its sums over the columns (gradient of a bias per row; no runs),
- * each NULL where it is not wanted.  act = identity: G is dC, pass NULL; pre is not read.  Then
- * dA = alpha G B' (DENSE / ROWS) and dB = alpha A' G (DENSE / SUM) are locus_hip_product_dev calls;
- * the gradient of res is beta dC.  Rows of no run: G is not written. */
-typedef struct locus_hip_product_slope_args {
-    int64_t m, n;
-    int32_t dtype, act;
+/* The gradient of that call, for dC (m x n) and the Z it kept in pre (not read for the identity):
+ *   G = dC act'(pre),  dA = alpha G B' (m x k),  dB = alpha A' G (k x n; ROWS: [groups][k][n], 0 for an
+ *   empty run),  col_sums[n] (ROWS: [groups][n]) = G summed over rows, the gradient of a bias per
+ *   column;  row_sums[m] (DENSE) = G summed over columns, of a bias per row;  G itself, of a whole matrix.
+ * Outputs are row-major, each NULL where it is not wanted; for the identity G is dC (pass NULL).  The
+ * gradient of res is beta dC.  ROWS: rows of no run are 0 in dA and not written in G; with gather dA
+ * stays in the order of the runs (the gradient of A's row i is the sum of the dA[r] with gather[r] = i). */
+typedef struct locus_hip_product_grad_args {
+    int64_t m, n, k;            /* of the forward call, and k <= 4194240                        */
+    int32_t dtype, act, mode, pad_;
+    int32_t cfg[2];             /* as there                                                     */
+    double alpha;
     const void* dC; int64_t sd_m, sd_n;
     const void* pre; int64_t sp_m, sp_n;
-    void* G;
-    void* col_sums;
-    void* row_sums;
-    int64_t groups; const int64_t* offsets;       /* 0, NULL: one run                           */
+    const void* A; int64_t sa_m, sa_k;
+    const void* B; int64_t sb_k, sb_n;
+    void* G; void* dA; void* dB; void* col_sums; void* row_sums;
+    int64_t groups; const int64_t* offsets; int64_t sb_g;
+    const int64_t* gather; int64_t a_rows;
     void* workspace; int64_t workspace_bytes;
-} locus_hip_product_slope_args;
-int locus_hip_product_slope_dev(const locus_hip_product_slope_args* args, void* stream);
-int64_t locus_hip_product_slope_workspace_bytes(const locus_hip_product_slope_args* args);
+} locus_hip_product_grad_args;
+int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* stream);
+/* Bytes of workspace (of the pointers only which are NULL is looked at), or a negative error. */
+int64_t locus_hip_product_grad_workspace_bytes(const locus_hip_product_grad_args* args);
 
 /* Element-wise part of coreBatch / coreZBatch / coreProbitBatch on [p][d] planes
  * (src/coreBatch.cpp:32-39):  T = X'(Y - M [- Zmu]) on entry in `mu` plane;

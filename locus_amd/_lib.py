@@ -106,8 +106,8 @@ SIGNATURES = {
     # fused and grouped products (products.py packs the argument structs)
     "locus_hip_product_dev": (_int, [_ptr, _ptr]),
     "locus_hip_product_workspace_bytes": (_i64, [_ptr]),
-    "locus_hip_product_slope_dev": (_int, [_ptr, _ptr]),
-    "locus_hip_product_slope_workspace_bytes": (_i64, [_ptr]),
+    "locus_hip_product_grad_dev": (_int, [_ptr, _ptr]),
+    "locus_hip_product_grad_workspace_bytes": (_i64, [_ptr]),
     # resident context (host pointers)
     "locus_hip_ctx_create": (_int, [_ptr, _ptr, _i64, _i64, _i64, ctypes.POINTER(_ptr)]),
     "locus_hip_ctx_set_state": (_int, [_ptr, _ptr, _ptr, _ptr]),

@@ -121,59 +121,47 @@ __device__ __forceinline__ void epi_store(const ProductEpi& e, long bias0, long 
 // ---- runs --------------------------------------------------------------------------------------
 struct Run {
     int g;            // which run (-1: none)
-    long lo, hi;      // its rows (of the tile asked for)
+    int lo, hi;       // its rows (of the tile asked for)
 };
 
-__device__ __forceinline__ long uniform_long(long v)
-{
-    const int lo = __builtin_amdgcn_readfirstlane((int)(v & 0xffffffff));
-    const int hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-    return ((long)hi << 32) | (unsigned)lo;
-}
-
-__device__ __forceinline__ long shfl_long(long v, int lane)
-{
-    const int lo = __shfl((int)(v & 0xffffffff), lane), hi = __shfl((int)(v >> 32), lane);
-    return ((long)hi << 32) | (unsigned)lo;
-}
+__device__ __forceinline__ int bounded(int64_t v, int rows) { return v < 0 ? 0 : (v > rows ? rows : (int)v); }
 
 // 64 offsets at a time, one per lane: the ordered offsets are a running maximum, the tiles before a
-// run a running sum.  Every wave does this for itself (no barrier); ~0.3 us for up to 64 runs,
+// run a running sum.  Every wave does this for itself (no barrier); under 1 us for up to 64 runs,
 // against a launch of its own for a tile map.  `tile` counts tiles of `bm` rows over all runs in
 // order; bm = 0 looks the run of row `tile` up instead.  first / last: the rows that runs cover.
-__device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, long rows, long tile,
-                                        int bm, long* first = nullptr, long* last = nullptr)
+__device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int rows, int tile, int bm,
+                                        int* first = nullptr, int* last = nullptr)
 {
     const int lane = threadIdx.x & 63;
-    auto bounded = [&](long v) { return v < 0 ? 0 : (v > rows ? rows : v); };
-    long carry = bounded(offsets[0]);
+    int carry = bounded(offsets[0], rows);
     if (first) *first = carry;
-    long before = 0;                                   // tiles of the runs before this chunk
+    int before = 0;                                    // tiles of the runs before this chunk
     Run found = {-1, 0, 0};
     for (int base = 0; base < groups; base += 64) {
         const int g = base + lane;
-        long hi = g < groups ? bounded(offsets[g + 1]) : 0;
+        int hi = g < groups ? bounded(offsets[g + 1], rows) : 0;
         hi = hi > carry ? hi : carry;
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
-            const long o = shfl_long(hi, lane - s);
+            const int o = __shfl_up(hi, s);
             if (lane >= s && o > hi) hi = o;
         }
-        const long up = shfl_long(hi, lane - 1);
-        const long lo = lane == 0 ? carry : up;
+        const int up = __shfl_up(hi, 1);
+        const int lo = lane == 0 ? carry : up;
         bool mine;
-        long excl = 0;
+        int excl = 0;
         if (bm) {
-            const long t = (hi - lo + bm - 1) / bm;
-            long incl = t;
+            const int t = (hi - lo + bm - 1) / bm;
+            int incl = t;
 #pragma unroll
             for (int s = 1; s < 64; s <<= 1) {
-                const long o = shfl_long(incl, lane - s);
+                const int o = __shfl_up(incl, s);
                 if (lane >= s) incl += o;
             }
             excl = before + incl - t;
             mine = tile >= excl && tile < before + incl;
-            before += shfl_long(incl, 63);
+            before += __shfl(incl, 63);
         } else {
             mine = tile >= lo && tile < hi;
         }
@@ -181,39 +169,38 @@ __device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, long
         if (hit && found.g < 0) {
             const int src = __ffsll((long long)hit) - 1;
             found.g = base + src;
-            const long rlo = shfl_long(lo, src), rhi = shfl_long(hi, src);
-            const long t0 = bm ? rlo + (tile - shfl_long(excl, src)) * bm : rlo;
+            const int rlo = __shfl(lo, src), rhi = __shfl(hi, src);
+            const int t0 = bm ? rlo + (tile - __shfl(excl, src)) * bm : rlo;
             found.lo = t0;
-            found.hi = bm && t0 + bm < rhi ? t0 + bm : rhi;
+            found.hi = bm && rhi - t0 > bm ? t0 + bm : rhi;
             if (!last) break;
         }
-        carry = shfl_long(hi, 63);
+        carry = __shfl(hi, 63);
     }
-    if (last) *last = uniform_long(carry);
+    if (last) *last = __builtin_amdgcn_readfirstlane(carry);
     found.g = __builtin_amdgcn_readfirstlane(found.g);
-    found.lo = uniform_long(found.lo);
-    found.hi = uniform_long(found.hi);
+    found.lo = __builtin_amdgcn_readfirstlane(found.lo);
+    found.hi = __builtin_amdgcn_readfirstlane(found.hi);
     return found;
 }
 
 // Rows [lo, hi) of one run by its number (the same ordered offsets).
-__device__ __forceinline__ Run run_rows(const int64_t* offsets, long rows, int g)
+__device__ __forceinline__ Run run_rows(const int64_t* offsets, int rows, int g)
 {
     const int lane = threadIdx.x & 63;
-    auto bounded = [&](long v) { return v < 0 ? 0 : (v > rows ? rows : v); };
-    long top = 0;                                      // largest of offsets[0 .. g]
+    int top = 0;                                       // largest of offsets[0 .. g]
     for (int i = lane; i <= g; i += 64) {
-        const long v = bounded(offsets[i]);
+        const int v = bounded(offsets[i], rows);
         top = v > top ? v : top;
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) {
-        const long o = shfl_long(top, lane ^ s);
+        const int o = __shfl_xor(top, s);
         top = o > top ? o : top;
     }
-    const long hi = bounded(offsets[g + 1]);
-    Run r = {g, uniform_long(top), 0};
-    r.hi = uniform_long(hi > top ? hi : top);
+    const int hi = bounded(offsets[g + 1], rows);
+    Run r = {g, __builtin_amdgcn_readfirstlane(top), 0};
+    r.hi = __builtin_amdgcn_readfirstlane(hi > top ? hi : top);
     return r;
 }
 
@@ -221,9 +208,9 @@ __device__ __forceinline__ Run run_rows(const int64_t* offsets, long rows, int g
 template <class T>
 __device__ __forceinline__ void fill_rest_rows(const ProductDesc& p, int n0, int n1)
 {
-    long first, last;
+    int first, last;
     find_run(p.offsets, p.groups, p.m, -1, 1, &first, &last);
-    const long outside = first + (p.m - last);
+    const long outside = (long)first + (p.m - last);
     const long w = n1 - n0;
     for (long e = threadIdx.x; e < outside * w; e += blockDim.x) {
         const long q = e / w, j = n0 + e % w;
@@ -253,8 +240,12 @@ template <> struct Mfma<float> {
 };
 
 // Launchers, one translation unit per type (product_f64.hip, product_f32.hip).  tw: 4 = tiles of
-// 128 x 128, 2 = 64 x 64; mt: 1, 2 or 4 times 16 rows.
+// 128 x 128, 2 = 64 x 64.  A pair is two independent products in one launch; false: not this pair.
 template <class T> int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st);
-template <class T> int launch_product_rows(const ProductDesc& p, int mode, int mt, hipStream_t st);
+template <class T> int launch_product_rows(const ProductDesc& p, int mode, hipStream_t st);
+template <class T>
+bool product_pairs(const ProductDesc& p, int mode, int tw, const ProductDesc& q, int qmode, int qtw);
+template <class T>
+int launch_product_pair(const ProductDesc& p, int mode, const ProductDesc& q, int tw, hipStream_t st);
 
 }  // namespace locus

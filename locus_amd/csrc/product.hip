@@ -38,18 +38,20 @@ __global__ void __launch_bounds__(256) product_join_kernel(const ProductDesc p)
 }
 
 // G = dC act'(pre) and the sums of its columns, per run and part of a run: bound by reading dC and
-// pre and writing G.  64 columns x 4 rows at a time; sums[part][groups][n], or dbias where there is one part.
+// pre and writing G.  64 columns x 16 rows at a time; sums[part][groups][n], or the column sums themselves where
+// there is one part.
 template <class T>
-__global__ void __launch_bounds__(256) product_slope_kernel(const locus_hip_product_slope_args a,
-                                                            int parts, T* sums)
+__global__ void __launch_bounds__(1024) product_slope_kernel(const locus_hip_product_grad_args a, T* G,
+                                                             int parts, T* sums)
 {
-    __shared__ T red[4][64];
+    constexpr int ROWS = 16;
+    __shared__ T red[ROWS][64];
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const long j = (long)blockIdx.x * 64 + tx;
     const int part = blockIdx.y, g = blockIdx.z;
     long lo = 0, hi = a.m;
     if (a.offsets) {
-        const Run r = run_rows(a.offsets, a.m, g);
+        const Run r = run_rows(a.offsets, (int)a.m, g);
         lo = r.lo;
         hi = r.hi;
     }
@@ -58,23 +60,31 @@ __global__ void __launch_bounds__(256) product_slope_kernel(const locus_hip_prod
     lo = lo + len * part / parts;
     T sum = T(0);
     if (j < a.n) {
-        const T* d = static_cast<const T*>(a.dC) + j * a.sd_n;
-        const T* z = static_cast<const T*>(a.pre) + j * a.sp_n;
-        T* out = static_cast<T*>(a.G) + j;
+        const T* d = static_cast<const T*>(a.dC) + j * a.sd_n + (lo + ty) * a.sd_m;
+        const T* z = static_cast<const T*>(a.pre) + j * a.sp_n + (lo + ty) * a.sp_m;
+        T* out = G + j + (lo + ty) * a.n;
+        const bool own = a.act != LOCUS_HIP_ACT_IDENTITY;
 #pragma unroll 4
-        for (long i = lo + ty; i < hi; i += 4) {
-            T v = d[i * a.sd_m];
-            if (a.act != LOCUS_HIP_ACT_IDENTITY) v *= act_slope<T>(a.act, z[i * a.sp_m]);
-            if (a.G) out[i * a.n] = v;
+        for (long i = lo + ty; i < hi; i += ROWS) {
+            T v = *d;
+            if (own) {
+                v *= act_slope<T>(a.act, *z);
+                *out = v;
+            }
             sum += v;
+            d += ROWS * a.sd_m;
+            z += ROWS * a.sp_m;
+            out += ROWS * a.n;
         }
     }
     if (sums == nullptr) return;
     red[ty][tx] = sum;
     __syncthreads();
     if (ty == 0 && j < a.n) {
-        const long at = ((long)part * gridDim.z + g) * a.n + j;
-        sums[at] = (red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]);
+        T v = red[0][tx];
+#pragma unroll
+        for (int q = 1; q < ROWS; ++q) v += red[q][tx];
+        sums[((long)part * gridDim.z + g) * a.n + j] = v;
     }
 }
 
@@ -108,122 +118,92 @@ __global__ void __launch_bounds__(256) product_row_sums_kernel(const T* G, long 
 unsigned grid_of(long want) { return (unsigned)std::max<long>(1, std::min<long>(want, 1 << 20)); }
 
 struct Plan {
-    int rows_mt = 0;     // > 0: the kernel for few rows, with so many 16-row tiles
-    int tw = 0;          // else: tiles of 32 tw
+    bool rows = false;   // the kernel for few rows
+    int tw = 4;          // else: tiles of 32 tw
     bool swap = false;   // C' = B' A' (n is the short side)
     int nz = 1;
     long kchunk = 0;
 };
 
-// Which kernel, tile and split.  Times in microseconds from rates measured on this card (tiles:
-// what a CU reaches with one and with several workgroups on it; joining: the partials written and
-// read at 4.5 TB/s and one more launch).
-Plan plan_product(const locus_hip_product_args& a)
+// One product: its operands and what is asked of the plan.
+struct Want {
+    ProductDesc p;
+    int mode;
+    bool f64;
+    int cfg[2];
+    long cus;            // CUs it may count on
+    long few;            // up to so many rows (or columns) take the kernel for few rows
+};
+
+// Which kernel, tile and split.  Times in microseconds from rates measured on this card (tiles: what a
+// CU reaches with one and with several workgroups on it; joining: the partials written and read at
+// 4.5 TB/s and one more launch).
+Plan plan_product(const Want& w)
 {
     Plan pl;
-    const bool f64 = a.dtype == LOCUS_HIP_F64;
-    const long s = f64 ? 8 : 4;
-    const long cus = device_cus();
-    const bool runs = a.mode == LOCUS_HIP_PRODUCT_ROWS;
-    const double avg = runs ? (double)a.m / a.groups : (double)a.m;
-    const long bk = f64 ? 16 : 32;
-    pl.kchunk = a.k;
-    if (a.mode == LOCUS_HIP_PRODUCT_SUM) {
-        const long t128 = ((a.m + 127) / 128) * ((a.n + 127) / 128) * a.groups;
-        pl.tw = a.cfg[0] ? a.cfg[0] / 32 : (t128 >= 2 * cus && a.m > 64 && a.n > 64 ? 4 : 2);
+    const ProductDesc& p = w.p;
+    const long M = p.m, N = p.n, K = p.k, s = w.f64 ? 8 : 4, bk = w.f64 ? 16 : 32;
+    const bool runs = w.mode == PRODUCT_ROWS;
+    const double avg = runs ? (double)M / p.groups : (double)M;
+    pl.kchunk = K;
+    if (w.mode == PRODUCT_SUM) {
+        const long t128 = ((M + 127) / 128) * ((N + 127) / 128) * p.groups;
+        pl.tw = w.cfg[0] >= 64 ? w.cfg[0] / 32 : (t128 >= 8 * w.cus ? 4 : 2);
         return pl;
     }
-    const long shortside = runs ? (long)avg : std::min(a.m, a.n);
-    const bool rows = a.cfg[0] ? a.cfg[0] <= 4 : shortside <= 64;
-    if (rows) {
-        pl.swap = !runs && a.n < a.m;
-        const long m = pl.swap ? a.n : a.m, n = pl.swap ? a.m : a.n;
-        const double per = runs ? avg : (double)m;
-        pl.rows_mt = a.cfg[0] ? a.cfg[0] : (per <= 16 ? 1 : (per <= 32 ? 2 : 4));
-        const long bm = 16 * pl.rows_mt, kb = f64 ? 8 : 16;
-        const long rt = runs ? std::max<long>(1, std::min<long>(a.m, a.m / bm + a.groups)) : (m + bm - 1) / bm;
+    const long side = runs ? (long)avg : std::min(M, N);
+    pl.rows = w.cfg[0] ? w.cfg[0] == 16 : side <= w.few;
+    if (pl.rows) {
+        pl.swap = !runs && N < M;
+        const long m = pl.swap ? N : M, n = pl.swap ? M : N, kb = w.f64 ? 8 : 16;
+        const long rt = runs ? std::max<long>(1, std::min<long>(m, m / 16 + p.groups)) : (m + 15) / 16;
         const long wgs = rt * ((n + 63) / 64);
-        long nz = std::min<long>(2 * cus / wgs, a.k / (16 * kb));
-        nz = std::min<long>(nz, std::max<long>(1, (long)(0.1 * a.k / per)));
-        if (a.cfg[1]) nz = a.cfg[1];
+        // two workgroups a CU; a wave gets 16 blocks of k at least (a launch to join costs as much), and the
+        // partials stay within a tenth of B
+        long nz = std::min<long>(2 * w.cus / wgs, K / (64 * kb));
+        nz = std::min<long>(nz, (long)(0.1 * K / (runs ? avg : (double)m)));
+        if (w.cfg[1]) nz = w.cfg[1];
         nz = std::max<long>(1, std::min<long>(nz, 256));
-        pl.kchunk = (a.k + nz - 1) / nz;
-        pl.kchunk = std::max<long>((pl.kchunk + 4 * kb - 1) / (4 * kb) * (4 * kb), 4 * kb);
-        pl.nz = (int)std::max<long>(1, (a.k + pl.kchunk - 1) / pl.kchunk);
+        pl.kchunk = ((K + nz - 1) / nz + 4 * kb - 1) / (4 * kb) * (4 * kb);
+        pl.nz = pl.kchunk > 0 ? (int)((K + pl.kchunk - 1) / pl.kchunk) : 1;
         return pl;
     }
-    const double cu_rate = (f64 ? 75e6 : 150e6) / cus;     // flop per us
+    const double cu_rate = (w.f64 ? 75e6 : 150e6) / w.cus;     // flop per us
     double best = 1e300;
     for (int tw = 4; tw >= 2; tw -= 2) {
-        if (a.cfg[0] && a.cfg[0] != 32 * tw) continue;
+        if (w.cfg[0] && w.cfg[0] != 32 * tw) continue;
         const long bm = 32 * tw;
-        const long mt = runs ? (long)(a.groups * ((long)(avg + bm - 1) / bm)) : (a.m + bm - 1) / bm;
-        const long tiles = std::max<long>(mt, 1) * ((a.n + bm - 1) / bm);
-        for (long nz = 1; nz <= 32; ++nz) {
-            if (a.cfg[1]) nz = a.cfg[1];
-            const long chunk = ((a.k + nz - 1) / nz + bk - 1) / bk * bk;
-            if (!a.cfg[1] && nz > 1 && chunk < 8 * bk) break;
-            const long used = a.k > 0 ? (a.k + chunk - 1) / chunk : 1;
-            const long wgs = tiles * used, load = (wgs + cus - 1) / cus;
-            const double eff = tw == 4 ? (load == 1 ? 0.7 : 0.92) : (load == 1 ? 0.5 : (load == 2 ? 0.7 : 0.8));
+        const long mt = runs ? p.groups * ((long)(avg + bm - 1) / bm) : (M + bm - 1) / bm;
+        const long tiles = std::max<long>(mt, 1) * ((N + bm - 1) / bm);
+        for (long nz = w.cfg[1] ? w.cfg[1] : 1; nz <= (w.cfg[1] ? w.cfg[1] : 32); ++nz) {
+            const long chunk = ((K + nz - 1) / nz + bk - 1) / bk * bk;
+            if (!w.cfg[1] && nz > 1 && chunk < 8 * bk) break;
+            const long used = K > 0 ? (K + chunk - 1) / chunk : 1;
+            const long wgs = tiles * used, load = (wgs + w.cus - 1) / w.cus;
+            const double eff = tw == 4 ? (load == 1 ? 0.7 : 0.92) : (load == 1 ? 0.6 : (load == 2 ? 0.75 : 0.87));
             double t = load * 2.0 * bm * bm * chunk / (cu_rate * eff);
-            if (used > 1) t += 4.0 + 2.0 * used * a.m * a.n * s / 4.5e6;
+            if (used > 1) t += 4.0 + 2.0 * used * M * N * s / 4.5e6;
             if (t < best) {
                 best = t;
                 pl.tw = tw;
                 pl.nz = (int)used;
                 pl.kchunk = chunk;
             }
-            if (a.cfg[1]) break;
         }
     }
-    if (pl.tw == 0) pl.tw = 4;
     return pl;
 }
 
-long plan_bytes(const locus_hip_product_args& a, const Plan& pl)
+long plan_bytes(const Want& w, const Plan& pl)
 {
-    return pl.nz > 1 ? (long)pl.nz * a.m * a.n * (a.dtype == LOCUS_HIP_F64 ? 8 : 4) : 0;
+    return pl.nz > 1 ? (long)pl.nz * w.p.m * w.p.n * (w.f64 ? 8 : 4) : 0;
 }
 
-int check_product(const locus_hip_product_args* a)
+// The descriptor as the kernels take it: roles swapped, split sum in `part`.
+ProductDesc planned(const Want& w, const Plan& pl, void* part)
 {
-    LOCUS_REQUIRE(a, "product: no arguments");
-    LOCUS_REQUIRE(a->dtype == LOCUS_HIP_F64 || a->dtype == LOCUS_HIP_F32, "product: dtype");
-    LOCUS_REQUIRE(a->act >= LOCUS_HIP_ACT_IDENTITY && a->act <= LOCUS_HIP_ACT_SILU, "product: act");
-    LOCUS_REQUIRE(a->mode >= LOCUS_HIP_PRODUCT_DENSE && a->mode <= LOCUS_HIP_PRODUCT_SUM, "product: mode");
-    LOCUS_REQUIRE(a->m >= 0 && a->n >= 0 && a->k >= 0 && a->m < (1ll << 30) && a->n <= 65535 * 64 &&
-                      a->k < (1ll << 30),
-                  "product: sizes (m, k < 2^30, n <= 4194240)");
-    LOCUS_REQUIRE(a->cfg[0] == 0 || a->cfg[0] == 64 || a->cfg[0] == 128 ||
-                      (a->mode != LOCUS_HIP_PRODUCT_SUM &&
-                       (a->cfg[0] == 1 || a->cfg[0] == 2 || a->cfg[0] == 4)),
-                  "product: cfg[0] is 0, 1, 2, 4, 64 or 128 (64 or 128 for a sum over runs)");
-    LOCUS_REQUIRE(a->cfg[1] >= 0 && a->cfg[1] <= 256 && (a->cfg[1] <= 1 || a->mode != LOCUS_HIP_PRODUCT_SUM),
-                  "product: cfg[1] is 0..256 (0 or 1 for a sum over runs)");
-    LOCUS_REQUIRE(a->cfg[0] == 0 || a->cfg[0] > 4 || a->mode != LOCUS_HIP_PRODUCT_DENSE ||
-                      std::min(a->m, a->n) < (1ll << 20),
-                  "product: the kernel for few rows takes fewer than 2^20 of them");
-    if (a->mode != LOCUS_HIP_PRODUCT_DENSE) {
-        LOCUS_REQUIRE(a->groups >= 1 && a->groups <= 65535, "product: groups (1..65535)");
-        LOCUS_REQUIRE(!a->gather || a->a_rows >= 0, "product: a_rows");
-    }
-    return 0;
-}
-
-template <class T>
-int run_product(const locus_hip_product_args& a, const Plan& pl, hipStream_t st)
-{
-    ProductDesc p = {};
-    p.m = (int)a.m; p.n = (int)a.n; p.k = (int)a.k;
-    p.A = a.A; p.sa_m = a.sa_m; p.sa_k = a.sa_k;
-    p.B = a.B; p.sb_k = a.sb_k; p.sb_n = a.sb_n;
+    ProductDesc p = w.p;
     ProductEpi& e = p.epi;
-    e.C = a.C; e.sc_m = a.sc_m; e.sc_n = a.sc_n;
-    e.bias = a.bias; e.sb_m = a.sbias_m; e.sb_n = a.sbias_n;
-    e.res = a.res; e.sr_m = a.sr_m; e.sr_n = a.sr_n;
-    e.pre = a.pre; e.sp_m = a.sp_m; e.sp_n = a.sp_n;
-    e.alpha = a.alpha; e.beta = a.beta; e.act = a.act;
     if (pl.swap) {
         std::swap(p.m, p.n);
         std::swap(p.A, p.B);
@@ -235,87 +215,216 @@ int run_product(const locus_hip_product_args& a, const Plan& pl, hipStream_t st)
         std::swap(e.sr_m, e.sr_n);
         std::swap(e.sp_m, e.sp_n);
     }
-    const int mode = a.mode;
-    if (mode != PRODUCT_DENSE) {
-        p.groups = (int)a.groups;
-        p.offsets = a.offsets;
-        p.sb_g = a.sb_g; p.sbias_g = a.sbias_g; p.sc_g = a.sc_g;
-        p.gather = a.gather;
-        p.a_rows = a.a_rows;
-        p.fill_rest = mode == PRODUCT_ROWS && a.fill_rest;
-    }
     p.nz = pl.nz;
     p.kchunk = (int)pl.kchunk;
     if (pl.nz > 1) {
-        p.part = a.workspace;
+        p.part = part;
         p.part_z = (long)p.m * p.n;
-        const bool mfast = mode == PRODUCT_DENSE && e.sc_n != 1 && e.sc_m == 1 && !pl.rows_mt;
+        const bool mfast = w.mode == PRODUCT_DENSE && e.sc_n != 1 && e.sc_m == 1 && !pl.rows;
         p.part_m = mfast ? 1 : p.n;
         p.part_n = mfast ? p.m : 1;
     }
-    int rc = pl.rows_mt ? launch_product_rows<T>(p, mode, pl.rows_mt, st)
-                        : launch_product_tile<T>(p, mode, pl.tw, st);
-    if (rc) return rc;
-    if (pl.nz > 1) {
-        if (mode == PRODUCT_DENSE)
-            hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_DENSE>),
-                               dim3(grid_of(((long)p.m * p.n + 255) / 256)), dim3(256), 0, st, p);
-        else
-            hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_ROWS>),
-                               dim3(grid_of(p.m), (unsigned)((p.n + 255) / 256)), dim3(256), 0, st, p);
-        LOCUS_HIP_CHECK(hipGetLastError());
+    return p;
+}
+
+template <class T> int join_product(const ProductDesc& p, int mode, hipStream_t st)
+{
+    if (p.nz <= 1) return 0;
+    if (mode == PRODUCT_DENSE)
+        hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_DENSE>), dim3(grid_of(((long)p.m * p.n + 255) / 256)),
+                           dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_ROWS>), dim3(grid_of(p.m), (unsigned)((p.n + 255) / 256)),
+                           dim3(256), 0, st, p);
+    LOCUS_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+template <class T> int run_product(const Want& w, const Plan& pl, void* part, hipStream_t st)
+{
+    if (w.p.m == 0 || w.p.n == 0) return 0;
+    const ProductDesc p = planned(w, pl, part);
+    const int rc = pl.rows ? launch_product_rows<T>(p, w.mode, st) : launch_product_tile<T>(p, w.mode, pl.tw, st);
+    return rc ? rc : join_product<T>(p, w.mode, st);
+}
+
+int check_common(const char* what, int64_t m, int64_t n, int64_t k, int dtype, int act, int mode, const int32_t* cfg,
+                 int64_t groups, const void* gather, int64_t a_rows)
+{
+    const std::string w(what);
+    LOCUS_REQUIRE(dtype == LOCUS_HIP_F64 || dtype == LOCUS_HIP_F32, w + ": dtype");
+    LOCUS_REQUIRE(act >= LOCUS_HIP_ACT_IDENTITY && act <= LOCUS_HIP_ACT_SILU, w + ": act");
+    LOCUS_REQUIRE(mode == LOCUS_HIP_PRODUCT_DENSE || mode == LOCUS_HIP_PRODUCT_ROWS, w + ": mode");
+    LOCUS_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < (1ll << 30) && n <= 65535 * 64 && k < (1ll << 30),
+                  w + ": sizes (m, k < 2^30, n <= 4194240)");
+    LOCUS_REQUIRE(cfg[0] == 0 || cfg[0] == 16 || cfg[0] == 64 || cfg[0] == 128, w + ": cfg[0] is 0, 16, 64 or 128");
+    LOCUS_REQUIRE(cfg[1] >= 0 && cfg[1] <= 256, w + ": cfg[1] is 0..256");
+    LOCUS_REQUIRE(cfg[0] != 16 || mode != LOCUS_HIP_PRODUCT_DENSE || std::min(m, n) < (1ll << 20),
+                  w + ": the kernel for few rows takes fewer than 2^20 of them");
+    if (mode == LOCUS_HIP_PRODUCT_ROWS) {
+        LOCUS_REQUIRE(groups >= 1 && groups <= 65535, w + ": groups (1..65535)");
+        LOCUS_REQUIRE(!gather || a_rows >= 0, w + ": a_rows");
     }
     return 0;
 }
 
-// Parts of a run whose column sums are taken side by side: about four workgroups per CU, runs of at
-// least 64 rows.
-int slope_parts(const locus_hip_product_slope_args& a)
+int check_product(const locus_hip_product_args* a)
+{
+    LOCUS_REQUIRE(a, "product: no arguments");
+    return check_common("product", a->m, a->n, a->k, a->dtype, a->act, a->mode, a->cfg, a->groups, a->gather, a->a_rows);
+}
+
+Want want_product(const locus_hip_product_args& a)
+{
+    Want w = {};
+    ProductDesc& p = w.p;
+    p.m = (int)a.m; p.n = (int)a.n; p.k = (int)a.k;
+    p.A = a.A; p.sa_m = a.sa_m; p.sa_k = a.sa_k;
+    p.B = a.B; p.sb_k = a.sb_k; p.sb_n = a.sb_n;
+    ProductEpi& e = p.epi;
+    e.C = a.C; e.sc_m = a.sc_m; e.sc_n = a.sc_n;
+    e.bias = a.bias; e.sb_m = a.sbias_m; e.sb_n = a.sbias_n;
+    e.res = a.res; e.sr_m = a.sr_m; e.sr_n = a.sr_n;
+    e.pre = a.pre; e.sp_m = a.sp_m; e.sp_n = a.sp_n;
+    e.alpha = a.alpha; e.beta = a.beta; e.act = a.act;
+    if (a.mode == LOCUS_HIP_PRODUCT_ROWS) {
+        p.groups = (int)a.groups;
+        p.offsets = a.offsets;
+        p.sb_g = a.sb_g; p.sbias_g = a.sbias_g;
+        p.gather = a.gather;
+        p.a_rows = a.a_rows;
+        p.fill_rest = a.fill_rest;
+    }
+    w.mode = a.mode;
+    w.f64 = a.dtype == LOCUS_HIP_F64;
+    w.cfg[0] = a.cfg[0]; w.cfg[1] = a.cfg[1];
+    w.cus = device_cus();
+    w.few = 48;
+    return w;
+}
+
+// ---- gradient ------------------------------------------------------------------------------------
+
+// Parts of a run whose column sums are taken side by side: about two workgroups (of 16 waves) per CU,
+// parts of at least 64 rows.
+int slope_parts(const locus_hip_product_grad_args& a)
 {
     const long blocks = ((a.n + 63) / 64) * std::max<long>(1, a.groups);
     const long per = a.m / std::max<long>(1, a.groups);
-    const long want = std::min<long>(4L * device_cus() / std::max<long>(1, blocks), per / 32);
+    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks), per / 64);
     return (int)std::max<long>(1, std::min<long>(want, 1024));
 }
 
-int check_slope(const locus_hip_product_slope_args* a)
+int check_grad(const locus_hip_product_grad_args* a)
 {
-    LOCUS_REQUIRE(a, "product_slope: no arguments");
-    LOCUS_REQUIRE(a->dtype == LOCUS_HIP_F64 || a->dtype == LOCUS_HIP_F32, "product_slope: dtype");
-    LOCUS_REQUIRE(a->act >= LOCUS_HIP_ACT_IDENTITY && a->act <= LOCUS_HIP_ACT_SILU, "product_slope: act");
-    LOCUS_REQUIRE(a->m >= 0 && a->n >= 0 && a->m < (1ll << 30) && a->n <= 65535 * 64,
-                  "product_slope: sizes (m < 2^30, n <= 4194240)");
-    LOCUS_REQUIRE(a->offsets ? a->groups >= 1 && a->groups <= 65535 : a->groups == 0,
-                  "product_slope: groups (1..65535 with offsets, else 0)");
-    LOCUS_REQUIRE(!(a->row_sums && a->offsets), "product_slope: row sums are for one run");
+    LOCUS_REQUIRE(a, "product_grad: no arguments");
+    int rc = check_common("product_grad", a->m, a->n, a->k, a->dtype, a->act, a->mode, a->cfg, a->groups, a->gather,
+                          a->a_rows);
+    if (rc) return rc;
+    LOCUS_REQUIRE(a->k <= 65535 * 64, "product_grad: sizes (k <= 4194240)");
+    LOCUS_REQUIRE(!(a->row_sums && a->mode == LOCUS_HIP_PRODUCT_ROWS), "product_grad: row sums are for one pair of matrices");
+    LOCUS_REQUIRE(!(a->G && a->act == LOCUS_HIP_ACT_IDENTITY), "product_grad: with act = identity, G is dC: pass NULL");
     return 0;
 }
 
-template <class T>
-int run_slope(const locus_hip_product_slope_args& a, hipStream_t st)
+// What a gradient launches: workspace [G | column sums | partials of dA | partials of dB].
+struct Grad {
+    bool own_g, slope;                 // G in the workspace; G or sums are asked for
+    int parts;
+    Want da, db;
+    Plan pa, pb;
+    long g_bytes, s_bytes, a_bytes, b_bytes;
+    long all() const { return g_bytes + s_bytes + a_bytes + b_bytes; }
+};
+
+Grad plan_grad(const locus_hip_product_grad_args& a)
 {
-    const unsigned groups = (unsigned)std::max<long>(1, a.groups);
-    if (a.G || a.col_sums) {
-        const int parts = slope_parts(a);
-        T* sums = a.col_sums ? (parts > 1 ? static_cast<T*>(a.workspace) : static_cast<T*>(a.col_sums)) : nullptr;
-        hipLaunchKernelGGL(product_slope_kernel<T>, dim3((unsigned)((a.n + 63) / 64), (unsigned)parts, groups),
-                           dim3(256), 0, st, a, parts, sums);
+    auto up = [](long v) { return (v + 255) / 256 * 256; };
+    Grad r = {};
+    const bool runs = a.mode == LOCUS_HIP_PRODUCT_ROWS, act = a.act != LOCUS_HIP_ACT_IDENTITY;
+    const long s = a.dtype == LOCUS_HIP_F64 ? 8 : 4;
+    r.own_g = act && !a.G;
+    r.slope = act || a.col_sums;
+    r.parts = slope_parts(a);
+    r.g_bytes = r.own_g ? up(a.m * a.n * s) : 0;
+    r.s_bytes = a.col_sums && r.parts > 1 ? up(r.parts * std::max<long>(1, a.groups) * a.n * s) : 0;
+    // G is row-major m x n, for the identity dC as it is
+    const long g_m = act ? a.n : a.sd_m, g_n = act ? 1 : a.sd_n;
+    Want w = {};
+    w.f64 = a.dtype == LOCUS_HIP_F64;
+    w.cfg[0] = a.cfg[0]; w.cfg[1] = a.cfg[1];
+    w.cus = a.dA && a.dB ? device_cus() / 2 : device_cus();
+    w.few = 16;
+    w.p.epi.alpha = a.alpha;
+    if (runs) {
+        w.p.groups = (int)a.groups;
+        w.p.offsets = a.offsets;
+    }
+    // dA = alpha G B'
+    r.da = w;
+    ProductDesc& p = r.da.p;
+    r.da.mode = a.mode;
+    p.m = (int)a.m; p.n = (int)a.k; p.k = (int)a.n;
+    p.sa_m = g_m; p.sa_k = g_n;
+    p.B = a.B; p.sb_k = a.sb_n; p.sb_n = a.sb_k; p.sb_g = a.sb_g;
+    p.epi.C = a.dA; p.epi.sc_m = a.k; p.epi.sc_n = 1;
+    p.fill_rest = runs;
+    // dB = alpha A' G, per run
+    r.db = w;
+    ProductDesc& q = r.db.p;
+    r.db.mode = runs ? PRODUCT_SUM : PRODUCT_DENSE;
+    q.m = (int)a.k; q.n = (int)a.n; q.k = (int)a.m;
+    q.A = a.A; q.sa_m = a.sa_k; q.sa_k = a.sa_m;
+    q.sb_k = g_m; q.sb_n = g_n;
+    q.epi.C = a.dB; q.epi.sc_m = a.n; q.epi.sc_n = 1;
+    q.sc_g = a.k * a.n;
+    if (runs) { q.gather = a.gather; q.a_rows = a.a_rows; }
+    if (a.dA) { r.pa = plan_product(r.da); r.a_bytes = up(plan_bytes(r.da, r.pa)); }
+    if (a.dB) { r.pb = plan_product(r.db); r.b_bytes = up(plan_bytes(r.db, r.pb)); }
+    return r;
+}
+
+template <class T> int run_grad(const locus_hip_product_grad_args& a, Grad& r, hipStream_t st)
+{
+    char* ws = static_cast<char*>(a.workspace);
+    const bool act = a.act != LOCUS_HIP_ACT_IDENTITY;
+    T* G = static_cast<T*>(r.own_g ? ws : a.G);
+    T* sums = static_cast<T*>(r.s_bytes ? ws + r.g_bytes : a.col_sums);
+    if (r.slope && a.n > 0) {
+        const unsigned groups = (unsigned)std::max<long>(1, a.groups);
+        hipLaunchKernelGGL(product_slope_kernel<T>, dim3((unsigned)((a.n + 63) / 64), (unsigned)r.parts, groups), dim3(1024),
+                           0, st, a, G, r.parts, sums);
         LOCUS_HIP_CHECK(hipGetLastError());
-        if (a.col_sums && parts > 1) {
+        if (r.s_bytes) {
             const long len = (long)groups * a.n;
-            hipLaunchKernelGGL(product_sums_join_kernel<T>, dim3((unsigned)((len + 255) / 256)), dim3(256), 0, st,
-                               sums, parts, len, static_cast<T*>(a.col_sums));
+            hipLaunchKernelGGL(product_sums_join_kernel<T>, dim3((unsigned)((len + 255) / 256)), dim3(256), 0, st, sums,
+                               r.parts, len, static_cast<T*>(a.col_sums));
             LOCUS_HIP_CHECK(hipGetLastError());
         }
     }
     if (a.row_sums && a.m > 0) {
-        const bool own = a.act != LOCUS_HIP_ACT_IDENTITY;
         hipLaunchKernelGGL(product_row_sums_kernel<T>, dim3(grid_of((a.m + 3) / 4)), dim3(256), 0, st,
-                           static_cast<const T*>(own ? a.G : a.dC), own ? a.n : a.sd_m, own ? 1L : a.sd_n, a.m,
-                           a.n, static_cast<T*>(a.row_sums));
+                           act ? G : static_cast<const T*>(a.dC), act ? a.n : a.sd_m, act ? 1L : a.sd_n, a.m, a.n,
+                           static_cast<T*>(a.row_sums));
         LOCUS_HIP_CHECK(hipGetLastError());
     }
-    return 0;
+    r.da.p.A = r.db.p.B = act ? G : a.dC;
+    void* const pa = ws + r.g_bytes + r.s_bytes;
+    void* const pb = ws + r.g_bytes + r.s_bytes + r.a_bytes;
+    const bool da = a.dA && a.m > 0 && a.k > 0, db = a.dB && a.k > 0 && a.n > 0;
+    if (da && db && !r.pa.rows && !r.pb.rows) {
+        const ProductDesc p = planned(r.da, r.pa, pa), q = planned(r.db, r.pb, pb);
+        if (product_pairs<T>(p, r.da.mode, r.pa.tw, q, r.db.mode, r.pb.tw)) {
+            int rc = launch_product_pair<T>(p, r.da.mode, q, r.pa.tw, st);
+            if (!rc) rc = join_product<T>(p, r.da.mode, st);
+            return rc ? rc : join_product<T>(q, r.db.mode, st);
+        }
+    }
+    if (da) {
+        const int rc = run_product<T>(r.da, r.pa, pa, st);
+        if (rc) return rc;
+    }
+    return db ? run_product<T>(r.db, r.pb, pb, st) : 0;
 }
 
 }  // namespace
@@ -329,8 +438,8 @@ int64_t locus_hip_product_workspace_bytes(const locus_hip_product_args* args)
 {
     const int rc = check_product(args);
     if (rc) return rc;
-    if (args->m == 0 || args->n == 0) return 0;
-    return plan_bytes(*args, plan_product(*args));
+    const Want w = want_product(*args);
+    return args->m == 0 || args->n == 0 ? 0 : plan_bytes(w, plan_product(w));
 }
 
 int locus_hip_product_dev(const locus_hip_product_args* args, void* stream)
@@ -343,36 +452,35 @@ int locus_hip_product_dev(const locus_hip_product_args* args, void* stream)
     LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || a.offsets, "product: runs need offsets");
     LOCUS_REQUIRE(a.pre != a.C, "product: pre and C are two buffers");
     LOCUS_REQUIRE(!a.gather || a.a_rows > 0 || a.k == 0, "product: rows gathered from an empty matrix");
-    const Plan pl = plan_product(a);
-    LOCUS_REQUIRE(plan_bytes(a, pl) <= (a.workspace ? a.workspace_bytes : 0),
+    const Want w = want_product(a);
+    const Plan pl = plan_product(w);
+    LOCUS_REQUIRE(plan_bytes(w, pl) <= (a.workspace ? a.workspace_bytes : 0),
                   "product: workspace smaller than locus_hip_product_workspace_bytes()");
-    return a.dtype == LOCUS_HIP_F64 ? run_product<double>(a, pl, (hipStream_t)stream)
-                                    : run_product<float>(a, pl, (hipStream_t)stream);
+    return w.f64 ? run_product<double>(w, pl, a.workspace, (hipStream_t)stream)
+                 : run_product<float>(w, pl, a.workspace, (hipStream_t)stream);
 }
 
-int64_t locus_hip_product_slope_workspace_bytes(const locus_hip_product_slope_args* args)
+int64_t locus_hip_product_grad_workspace_bytes(const locus_hip_product_grad_args* args)
 {
-    const int rc = check_slope(args);
-    if (rc) return rc;
-    const int parts = slope_parts(*args);
-    return parts > 1 ? (int64_t)parts * std::max<int64_t>(1, args->groups) * args->n *
-                           (args->dtype == LOCUS_HIP_F64 ? 8 : 4)
-                     : 0;
+    const int rc = check_grad(args);
+    return rc ? rc : plan_grad(*args).all();
 }
 
-int locus_hip_product_slope_dev(const locus_hip_product_slope_args* args, void* stream)
+int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* stream)
 {
-    int rc = check_slope(args);
+    int rc = check_grad(args);
     if (rc) return rc;
-    const locus_hip_product_slope_args& a = *args;
-    if (a.n == 0) return 0;
-    const bool identity = a.act == LOCUS_HIP_ACT_IDENTITY;
-    LOCUS_REQUIRE(a.m == 0 || (a.dC && (identity || (a.pre && a.G))), "product_slope: null pointer");
-    LOCUS_REQUIRE(!a.col_sums || locus_hip_product_slope_workspace_bytes(args) <=
-                                     (a.workspace ? a.workspace_bytes : 0),
-                  "product_slope: workspace smaller than locus_hip_product_slope_workspace_bytes()");
-    return a.dtype == LOCUS_HIP_F64 ? run_slope<double>(a, (hipStream_t)stream)
-                                    : run_slope<float>(a, (hipStream_t)stream);
+    const locus_hip_product_grad_args& a = *args;
+    const bool act = a.act != LOCUS_HIP_ACT_IDENTITY;
+    LOCUS_REQUIRE(a.m == 0 || a.n == 0 || (a.dC && (!act || a.pre)), "product_grad: null pointer");
+    LOCUS_REQUIRE(!a.dA || a.B || a.k == 0 || a.n == 0 || a.m == 0, "product_grad: dA needs B");
+    LOCUS_REQUIRE(!a.dB || a.A || a.k == 0 || a.n == 0 || a.m == 0, "product_grad: dB needs A");
+    LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || a.offsets, "product_grad: runs need offsets");
+    LOCUS_REQUIRE(!a.gather || a.a_rows > 0 || a.m == 0 || a.k == 0, "product_grad: rows gathered from an empty matrix");
+    Grad r = plan_grad(a);
+    LOCUS_REQUIRE(r.all() <= (a.workspace ? a.workspace_bytes : 0),
+                  "product_grad: workspace smaller than locus_hip_product_grad_workspace_bytes()");
+    return a.dtype == LOCUS_HIP_F64 ? run_grad<double>(a, r, (hipStream_t)stream) : run_grad<float>(a, r, (hipStream_t)stream);
 }
 
 }  // extern "C"

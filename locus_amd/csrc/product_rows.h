@@ -1,8 +1,10 @@
-// Matrix product of few rows (up to 16 MT = 16, 32 or 64 per tile) with the epilogue of ProductEpi:
-// one new sample against all effects, a served batch, runs of a few rows each.  B is read once (per
-// tile of rows) and bounds the time; the matrix cores take the products whatever the number of rows.
+// Matrix product of few rows (tiles of 16) with the epilogue of ProductEpi: one new sample against all
+// effects, a served batch, runs of a few rows each.  B is read once (per tile of rows) and bounds the
+// time; the matrix cores take the products whatever the number of rows.  (Tiles of 32 and 64 rows
+// that load B once for all of them are no faster: 33 samples x 20 011 x 1000 float32 33 us with three tiles
+// of 16, whose second and third reading of B comes from L2, 37 and 35 with the larger ones.)
 //
-// A workgroup of four waves owns 16 MT rows x 64 columns and a slice of k; its waves take a quarter
+// A workgroup of four waves owns 16 rows x 64 columns and a slice of k; its waves take a quarter
 // of the slice each and are added through LDS, the slices by product_join_kernel (or, where there is
 // one slice, the epilogue runs here).  Nothing of B passes through LDS: a lane loads 16 bytes at a time
 // straight into operand registers, DEPTH blocks ahead (16 loads of a wave in flight; two workgroups a
@@ -31,7 +33,7 @@ template <class T> struct Vec16 {
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-template <class T, int MT, int BKIND, int MODE>
+template <class T, int BKIND, int MODE>
 __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
 {
     constexpr int V = Vec16<T>::V;
@@ -40,8 +42,8 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
     constexpr int NT = 4;                   // column tiles of 16
     constexpr int UN = NT / V;              // loads side by side over the 64 columns
     constexpr int KB = 4 * V;               // k per block
-    constexpr int DEPTH = MT == 4 ? 2 : 4;  // blocks in flight
-    constexpr int BM = 16 * MT;
+    constexpr int DEPTH = 4;                // blocks in flight
+    constexpr int BM = 16;
     constexpr int EL = 65;
     __shared__ T lds[4 * 16 * EL];
 
@@ -78,20 +80,12 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
     const int kEnd = kb + per < kzEnd ? kb + per : kzEnd;
 
     // lane's rows of A (beyond the last row: the last one, never stored) and columns of B
-    const T* ap[MT];
-    bool bad[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        long row = m0 + t * 16 + c;
-        row = row < mEnd ? row : mEnd - 1;
-        bad[t] = false;
-        if (MODE == PRODUCT_ROWS && p.gather) {
-            row = p.gather[row];
-            bad[t] = row < 0 || row >= p.a_rows;
-            if (bad[t]) row = 0;
-        }
-        ap[t] = A + row * p.sa_m;
+    long row = m0 + c < mEnd ? m0 + c : mEnd - 1;
+    if (MODE == PRODUCT_ROWS && p.gather) {
+        row = p.gather[row];
+        if (row < 0 || row >= p.a_rows) row = 0;         // the epilogue makes it NaN
     }
+    const T* ap = A + row * p.sa_m;
     const bool a_vec = p.sa_k == 1;
     int first[UN];                              // BK_N: first column of the lane's load
     const T* bp[BKIND == ROWS_BK_N ? UN : NT];
@@ -110,13 +104,11 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
         }
     }
 
-    acc_t acc[MT][NT];
+    acc_t acc[NT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[t][j] = (acc_t){0, 0, 0, 0};
+    for (int j = 0; j < NT; ++j) acc[j] = (acc_t){0, 0, 0, 0};
 
-    T a[DEPTH][MT][V], b[DEPTH][NT][V];         // b[..][j][u]: column tile j, instruction u
+    T a[DEPTH][V], b[DEPTH][NT][V];             // b[..][j][u]: column tile j, instruction u
     auto load = [&](int s, int k0) {            // a whole block
         const int k = k0 + V * g;
         if constexpr (BKIND == ROWS_BK_N) {
@@ -142,17 +134,12 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
                 for (int u = 0; u < V; ++u) b[s][j][u] = bp[j][(long)(k + u) * p.sb_k];
         }
         if (a_vec) {
+            const vec_t x = *reinterpret_cast<const vec_t*>(ap + k);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const vec_t x = *reinterpret_cast<const vec_t*>(ap[t] + k);
-#pragma unroll
-                for (int u = 0; u < V; ++u) a[s][t][u] = x[u];
-            }
+            for (int u = 0; u < V; ++u) a[s][u] = x[u];
         } else {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int u = 0; u < V; ++u) a[s][t][u] = ap[t][(long)(k + u) * p.sa_k];
+            for (int u = 0; u < V; ++u) a[s][u] = ap[(long)(k + u) * p.sa_k];
         }
     };
     auto load_part = [&](int s, int k0) {       // the last, partial block: k beyond the end are 0
@@ -169,18 +156,14 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
                 }
                 b[s][j][u] = x;
             }
-#pragma unroll
-            for (int t = 0; t < MT; ++t) a[s][t][u] = in ? ap[t][(long)k * p.sa_k] : T(0);
+            a[s][u] = in ? ap[(long)k * p.sa_k] : T(0);
         }
     };
     auto use = [&](int s) {
 #pragma unroll
         for (int u = 0; u < V; ++u)
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc[t][j] = Mfma<T>::run(a[s][t][u], b[s][j][u], acc[t][j]);
+            for (int j = 0; j < NT; ++j) acc[j] = Mfma<T>::run(a[s][u], b[s][j][u], acc[j]);
     };
     if (kb < kEnd) {
         const int blocks = (kEnd - kb) / KB;            // whole ones
@@ -212,76 +195,61 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
         }
     }
 
-    // the four waves' sums, 16 rows at a time
+    // the four waves' sums
     constexpr int WS = 16 * EL;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        if (t) __syncthreads();
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            int col;                                     // in the tile
-            bool own = true;
-            if constexpr (BKIND == ROWS_BK_N) {
-                col = first[j / V] + j % V - n0;
-                own = col >= 16 * V * (j / V) + V * c;
-            } else {
-                col = 16 * j + c;
-            }
-            if (own)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    lds[wave * WS + Mfma<T>::row(lane, r) * EL + col] = acc[t][j][r];
+    for (int j = 0; j < NT; ++j) {
+        int col;                                         // in the tile
+        bool own = true;
+        if constexpr (BKIND == ROWS_BK_N) {
+            col = first[j / V] + j % V - n0;
+            own = col >= 16 * V * (j / V) + V * c;
+        } else {
+            col = 16 * j + c;
         }
-        __syncthreads();
+        if (own)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds[wave * WS + Mfma<T>::row(lane, r) * EL + col] = acc[j][r];
+    }
+    __syncthreads();
 #pragma unroll 1
-        for (int e = tid; e < 16 * 64; e += 256) {
-            const int i = e >> 6, j = e & 63;
-            const long gi = m0 + t * 16 + i;
-            const int gj = n0 + j;
-            if (gi < mEnd && gj < p.n) {
-                const T* x = lds + i * EL + j;
-                T v = (x[0] + x[WS]) + (x[2 * WS] + x[3 * WS]);
-                if (MODE == PRODUCT_ROWS && p.gather && p.k > 0) {
-                    const long row = p.gather[gi];
-                    if (row < 0 || row >= p.a_rows) v = T(__builtin_nan(""));
-                }
-                if (p.part)
-                    static_cast<T*>(p.part)[blockIdx.z * p.part_z + gi * p.part_m + gj * p.part_n] = v;
-                else
-                    epi_store<T>(p.epi, bias0, gi, gj, v);
+    for (int e = tid; e < 16 * 64; e += 256) {
+        const int i = e >> 6, j = e & 63;
+        const long gi = m0 + i;
+        const int gj = n0 + j;
+        if (gi < mEnd && gj < p.n) {
+            const T* x = lds + i * EL + j;
+            T v = (x[0] + x[WS]) + (x[2 * WS] + x[3 * WS]);
+            if (MODE == PRODUCT_ROWS && p.gather && p.k > 0) {
+                const long at = p.gather[gi];
+                if (at < 0 || at >= p.a_rows) v = T(__builtin_nan(""));
             }
+            if (p.part)
+                static_cast<T*>(p.part)[blockIdx.z * p.part_z + gi * p.part_m + gj * p.part_n] = v;
+            else
+                epi_store<T>(p.epi, bias0, gi, gj, v);
         }
     }
 }
 
 template <class T>
-int launch_product_rows(const ProductDesc& p, int mode, int mt, hipStream_t st)
+int launch_product_rows(const ProductDesc& p, int mode, hipStream_t st)
 {
     constexpr int V = Vec16<T>::V;
-    const int bm = 16 * mt;
     const unsigned gx = (unsigned)((p.n + 63) / 64);
-    const unsigned gy = mode == PRODUCT_DENSE ? (unsigned)((p.m + bm - 1) / bm)
-                                              : (unsigned)(p.m / bm + p.groups + (p.fill_rest ? 1 : 0));
+    const unsigned gy = mode == PRODUCT_DENSE ? (unsigned)((p.m + 15) / 16)
+                                              : (unsigned)(p.m / 16 + p.groups + (p.fill_rest ? 1 : 0));
     const int kind = p.sb_n == 1 && p.n >= V ? ROWS_BK_N : (p.sb_k == 1 ? ROWS_BK_K : ROWS_BK_ANY);
-    auto go = [&](auto kern) {
-        const bool dense = mode == PRODUCT_DENSE;
-        hipLaunchKernelGGL(kern, dim3(dense ? gx : gy, dense ? gy : gx, (unsigned)p.nz), dim3(256), 0, st, p);
-        return 0;
+    const bool dense = mode == PRODUCT_DENSE;
+    auto pick = [&](auto kc) {
+        constexpr int KIND = decltype(kc)::value;
+        const dim3 grid(dense ? gx : gy, dense ? gy : gx, (unsigned)p.nz);
+        if (dense) hipLaunchKernelGGL((product_rows_kernel<T, KIND, PRODUCT_DENSE>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((product_rows_kernel<T, KIND, PRODUCT_ROWS>), grid, dim3(256), 0, st, p);
     };
-    auto pick2 = [&](auto mtc, auto kc) {
-        constexpr int MT = decltype(mtc)::value, KIND = decltype(kc)::value;
-        return mode == PRODUCT_DENSE ? go(product_rows_kernel<T, MT, KIND, PRODUCT_DENSE>)
-                                     : go(product_rows_kernel<T, MT, KIND, PRODUCT_ROWS>);
-    };
-    auto pick = [&](auto mtc) {
-        if (kind == ROWS_BK_N) return pick2(mtc, std::integral_constant<int, ROWS_BK_N>{});
-        if (kind == ROWS_BK_K) return pick2(mtc, std::integral_constant<int, ROWS_BK_K>{});
-        return pick2(mtc, std::integral_constant<int, ROWS_BK_ANY>{});
-    };
-    const int rc = mt == 1 ? pick(std::integral_constant<int, 1>{})
-                           : (mt == 2 ? pick(std::integral_constant<int, 2>{})
-                                      : pick(std::integral_constant<int, 4>{}));
-    if (rc) return rc;
+    if (kind == ROWS_BK_N) pick(std::integral_constant<int, ROWS_BK_N>{});
+    else if (kind == ROWS_BK_K) pick(std::integral_constant<int, ROWS_BK_K>{});
+    else pick(std::integral_constant<int, ROWS_BK_ANY>{});
     LOCUS_HIP_CHECK(hipGetLastError());
     return 0;
 }

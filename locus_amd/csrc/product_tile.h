@@ -173,14 +173,15 @@ __device__ __forceinline__ void store_block(const ProductDesc& p, const T* lds, 
 // or the general form: run-time layouts and 64-bit lane addresses.
 enum { LAY_ANY = 0, LAY_FAST = 1, LAY_A_K = 2, LAY_B_K = 4 };
 
+// Workgroup `lin` of a grid of gx x gy x gz.
 template <class T, int TW, int BK, int PF, int MODE, int LAY>
-__global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(const ProductDesc p)
+__device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsigned lin, unsigned gx,
+                                             unsigned gy, unsigned gz)
 {
     typedef TileGeom<T, TW, BK> G;
     typedef typename Mfma<T>::acc_t acc_t;
     constexpr int BM = G::BM, BN = G::BN, LD = G::LD, NQ = G::NQ, BUF = G::BUF;
     constexpr bool FAST = LAY & LAY_FAST, AKF = LAY & LAY_A_K, BKF = LAY & LAY_B_K;
-    __shared__ T lds[G::ELEMS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave >> 1, wn = wave & 1;
@@ -190,8 +191,7 @@ __global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(cons
     // one slice of k, so that strips of A and B are read from its L2 by the others.
     unsigned bx, by, bz;
     {
-        const unsigned gx = gridDim.x, gy = gridDim.y, each = gx * gy, total = each * gridDim.z;
-        const unsigned lin = blockIdx.x + gx * (blockIdx.y + gy * blockIdx.z);
+        const unsigned each = gx * gy, total = each * gz;
         const unsigned xcd = lin & 7, rem = total & 7;
         const unsigned w = xcd * (total >> 3) + (xcd < rem ? xcd : rem) + (lin >> 3);
         bz = w / each;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(cons
         m0 = (long)bx * BM;
         mEnd = p.m;
     } else if constexpr (MODE == PRODUCT_ROWS) {
-        if (p.fill_rest && bx == gridDim.x - 1) {
+        if (p.fill_rest && bx == gx - 1) {
             if (bz == 0) fill_rest_rows<T>(p, n0, n0 + BN < p.n ? n0 + BN : p.n);
             return;
         }
@@ -444,53 +444,131 @@ __global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(cons
     }
 }
 
-template <class T>
-int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
+template <class T> constexpr int tile_bk() { return sizeof(T) == 8 ? 16 : 32; }
+template <class T, int TW> constexpr int tile_elems() { return TileGeom<T, TW, tile_bk<T>()>::ELEMS; }
+
+template <class T, int TW, int PF, int MODE, int LAY>
+__global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_tile_kernel(const ProductDesc p)
 {
-    constexpr int BK = sizeof(T) == 8 ? 16 : 32;
-    int bm = 32 * tw;
+    __shared__ T lds[tile_elems<T, TW>()];
+    product_tile<T, TW, tile_bk<T>(), PF, MODE, LAY>(
+        p, lds, blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), gridDim.x, gridDim.y, gridDim.z);
+}
+
+struct TileGrid {
+    unsigned x, y, z;
+    __host__ __device__ unsigned all() const { return (x * y * z + 7) / 8 * 8; }    // whole turns over the XCDs
+};
+struct ProductPair {
+    ProductDesc p, q;
+    TileGrid gp, gq;
+};
+
+// Two products that do not wait for each other (the two of a gradient) in one launch: the second one's
+// workgroups fill the CUs that the first one's last ones leave.
+template <class T, int TW, int MODE0, int LAY0, int MODE1, int LAY1>
+__global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_pair_kernel(const ProductPair d)
+{
+    __shared__ T lds[tile_elems<T, TW>()];
+    constexpr int PF = TW == 2 ? 2 : 1;
+    const unsigned first = d.gp.all();
+    const unsigned lin = blockIdx.x < first ? blockIdx.x : blockIdx.x - first;
+    if (blockIdx.x < first) {
+        if (lin < d.gp.x * d.gp.y * d.gp.z)
+            product_tile<T, TW, tile_bk<T>(), PF, MODE0, LAY0>(d.p, lds, lin, d.gp.x, d.gp.y, d.gp.z);
+    } else if (lin < d.gq.x * d.gq.y * d.gq.z) {
+        product_tile<T, TW, tile_bk<T>(), PF, MODE1, LAY1>(d.q, lds, lin, d.gq.x, d.gq.y, d.gq.z);
+    }
+}
+
+// The form a product takes: FAST and its layout, or LAY_ANY.  Compiled fast: every layout of one matrix pair;
+// runs of rows with A contiguous along a row; sums over runs with both operands contiguous along theirs.
+template <class T> int tile_layout(const ProductDesc& p, int mode, int tw)
+{
+    constexpr int BK = tile_bk<T>();
+    const int bm = 32 * tw;
     // 32-bit lane offsets: a K-tile's elements lie within 2^31 bytes behind its first one (a gathered
     // A: all of A does)
     const long lim = ((1L << 31) - 1) / (long)sizeof(T);
-    const long a_m = mode == PRODUCT_ROWS && p.gather ? p.a_rows : bm, a_k = mode == PRODUCT_SUM && p.gather ? p.a_rows : BK;
+    const long a_m = mode == PRODUCT_ROWS && p.gather ? p.a_rows : bm;
+    const long a_k = mode == PRODUCT_SUM && p.gather ? p.a_rows : BK;
     const bool off32 = p.sa_m >= 0 && p.sa_k >= 0 && p.sb_n >= 0 && p.sb_k >= 0 &&
                        (a_m - 1) * p.sa_m + (a_k - 1) * p.sa_k <= lim &&
                        (bm - 1) * p.sb_n + (BK - 1) * p.sb_k <= lim;
-    // Compiled fast: every layout of one matrix pair; runs of rows with A contiguous along a row; sums over
-    // runs with both operands contiguous along theirs.  The rest takes the general form (tiles of 64).
     const bool ak = p.sa_k == 1, bk = p.sb_k == 1;
-    const bool fast = off32 && (mode == PRODUCT_DENSE || (mode == PRODUCT_ROWS ? ak : !bk && (!ak || p.gather)));
-    if (!fast) bm = 64;
-    const unsigned gy = (unsigned)((p.n + bm - 1) / bm);
-    unsigned gx = (unsigned)((p.m + bm - 1) / bm), gz = p.part ? (unsigned)p.nz : 1u;
+    if (!off32 || (mode == PRODUCT_ROWS && !ak) || (mode == PRODUCT_SUM && (bk || (ak && !p.gather)))) return LAY_ANY;
+    return LAY_FAST | (ak && mode != PRODUCT_SUM ? LAY_A_K : 0) | (bk ? LAY_B_K : 0);
+}
+
+inline TileGrid tile_grid(const ProductDesc& p, int mode, int bm)
+{
+    TileGrid g = {(unsigned)((p.m + bm - 1) / bm), (unsigned)((p.n + bm - 1) / bm), p.part ? (unsigned)p.nz : 1u};
     // runs of rows: at most m / bm full tiles and one partial tile per run
-    if (mode == PRODUCT_ROWS) gx = (unsigned)(p.m / bm + p.groups + (p.fill_rest ? 1 : 0));
-    if (mode == PRODUCT_SUM) gz = (unsigned)p.groups;
-    auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3(gx, gy, gz), dim3(256), 0, st, p);
-        return 0;
-    };
+    if (mode == PRODUCT_ROWS) g.x = (unsigned)(p.m / bm + p.groups + (p.fill_rest ? 1 : 0));
+    if (mode == PRODUCT_SUM) g.z = (unsigned)p.groups;
+    return g;
+}
+
+template <class T>
+int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
+{
+    const int lay = tile_layout<T>(p, mode, tw);
+    const TileGrid g = tile_grid(p, mode, lay ? 32 * tw : 64);
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(g.x, g.y, g.z), dim3(256), 0, st, p); };
     auto pick = [&](auto twc) {
         constexpr int TW = decltype(twc)::value, PF = TW == 2 ? 2 : 1;
+        constexpr int AK = LAY_FAST | LAY_A_K, BK = LAY_FAST | LAY_B_K;
         if (mode == PRODUCT_DENSE) {
-            if (ak)
-                return bk ? go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST | LAY_A_K | LAY_B_K>)
-                          : go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST | LAY_A_K>);
-            return bk ? go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST | LAY_B_K>)
-                      : go(product_tile_kernel<T, TW, BK, PF, PRODUCT_DENSE, LAY_FAST>);
+            if (lay == (AK | BK)) go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, AK | BK>);
+            else if (lay == AK) go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, AK>);
+            else if (lay == BK) go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, BK>);
+            else go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, LAY_FAST>);
+        } else if (mode == PRODUCT_ROWS) {
+            if (lay == (AK | BK)) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK | BK>);
+            else go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK>);
+        } else {
+            go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST>);
         }
-        if (mode == PRODUCT_ROWS)
-            return bk ? go(product_tile_kernel<T, TW, BK, PF, PRODUCT_ROWS, LAY_FAST | LAY_A_K | LAY_B_K>)
-                      : go(product_tile_kernel<T, TW, BK, PF, PRODUCT_ROWS, LAY_FAST | LAY_A_K>);
-        return go(product_tile_kernel<T, TW, BK, PF, PRODUCT_SUM, LAY_FAST>);
     };
-    auto any = [&]() {
-        if (mode == PRODUCT_DENSE) return go(product_tile_kernel<T, 2, BK, 1, PRODUCT_DENSE, LAY_ANY>);
-        if (mode == PRODUCT_ROWS) return go(product_tile_kernel<T, 2, BK, 1, PRODUCT_ROWS, LAY_ANY>);
-        return go(product_tile_kernel<T, 2, BK, 1, PRODUCT_SUM, LAY_ANY>);
-    };
-    const int rc = !fast ? any() : tw == 4 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 2>{});
-    if (rc) return rc;
+    if (lay == LAY_ANY) {                       // tiles of 64 only
+        if (mode == PRODUCT_DENSE) go(product_tile_kernel<T, 2, 1, PRODUCT_DENSE, LAY_ANY>);
+        else if (mode == PRODUCT_ROWS) go(product_tile_kernel<T, 2, 1, PRODUCT_ROWS, LAY_ANY>);
+        else go(product_tile_kernel<T, 2, 1, PRODUCT_SUM, LAY_ANY>);
+    } else if (tw == 4) {
+        pick(std::integral_constant<int, 4>{});
+    } else {
+        pick(std::integral_constant<int, 2>{});
+    }
+    LOCUS_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+// Pairs that are compiled: a gradient's two products of row-major operands, dA = G B' and dB = A' G.
+template <class T>
+bool product_pairs(const ProductDesc& p, int mode, int tw, const ProductDesc& q, int qmode, int qtw)
+{
+    constexpr int ABK = LAY_FAST | LAY_A_K | LAY_B_K;
+    const TileGrid g = tile_grid(p, mode, 32 * tw), h = tile_grid(q, qmode, 32 * tw);
+    const double all = (double)g.x * g.y * g.z + (double)h.x * h.y * h.z;
+    return tw == qtw && all < (1 << 23) && (mode == PRODUCT_DENSE ? qmode == PRODUCT_DENSE : mode == PRODUCT_ROWS && qmode == PRODUCT_SUM) &&
+           tile_layout<T>(p, mode, tw) == ABK && tile_layout<T>(q, qmode, tw) == LAY_FAST;
+}
+
+template <class T>
+int launch_product_pair(const ProductDesc& p, int mode, const ProductDesc& q, int tw, hipStream_t st)
+{
+    constexpr int ABK = LAY_FAST | LAY_A_K | LAY_B_K;
+    const int qmode = mode == PRODUCT_DENSE ? PRODUCT_DENSE : PRODUCT_SUM;
+    const ProductPair d = {p, q, tile_grid(p, mode, 32 * tw), tile_grid(q, qmode, 32 * tw)};
+    const dim3 grid(d.gp.all() + d.gq.all());
+    if (mode == PRODUCT_DENSE && tw == 2)
+        hipLaunchKernelGGL((product_pair_kernel<T, 2, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>), grid, dim3(256), 0, st, d);
+    else if (mode == PRODUCT_DENSE)
+        hipLaunchKernelGGL((product_pair_kernel<T, 4, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>), grid, dim3(256), 0, st, d);
+    else if (tw == 2)
+        hipLaunchKernelGGL((product_pair_kernel<T, 2, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST>), grid, dim3(256), 0, st, d);
+    else
+        hipLaunchKernelGGL((product_pair_kernel<T, 4, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST>), grid, dim3(256), 0, st, d);
     LOCUS_HIP_CHECK(hipGetLastError());
     return 0;
 }

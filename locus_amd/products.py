@@ -28,9 +28,9 @@ from . import _lib
 
 ACTS = {"identity": 0, "logistic": 1, "probit": 2, "softplus": 3, "gelu": 4, "silu": 5}
 _DTYPES = {torch.float64: 0, torch.float32: 1}
-_DENSE, _ROWS, _SUM = 0, 1, 2
-_ARGS = struct.Struct("=3q6i2d27q")              # struct locus_hip_product_args
-_SLOPE_ARGS = struct.Struct("=2q2i13q")          # struct locus_hip_product_slope_args
+_DENSE, _ROWS = 0, 1
+_ARGS = struct.Struct("=3q6i2d26q")              # struct locus_hip_product_args
+_GRAD_ARGS = struct.Struct("=3q6id24q")          # struct locus_hip_product_grad_args
 
 
 def _fail(msg):
@@ -112,22 +112,25 @@ def _index(name, t, like, size):
         _fail(f"{name} must be contiguous")
 
 
-def _run(dev, fields, like):
-    """fields: of locus_hip_product_args up to the workspace."""
-    lib = _lib.lib()
-    need = lib.locus_hip_product_workspace_bytes(_ARGS.pack(*fields, 0, 0))
+def _run(pack, need_fn, run_fn, fields, like):
+    """One call of the library: `fields` of the argument struct up to the workspace."""
+    need = need_fn(pack(*fields, 0, 0))
     if need < 0:
         _lib.check(int(need))
-    ws = 0
+    dev, ws = like.device, None
     if need:
-        buf = torch.empty(need, dtype=torch.uint8, device=like.device)
-        ws = buf.data_ptr()
-    args = _ARGS.pack(*fields, ws, need)
-    if dev == torch.cuda.current_device():
-        _lib.check(lib.locus_hip_product_dev(args, torch.cuda.current_stream(dev).cuda_stream))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    args = pack(*fields, ws.data_ptr() if need else 0, need)
+    if dev.index == torch.cuda.current_device():
+        _lib.check(run_fn(args, torch.cuda.current_stream(dev).cuda_stream))
     else:
         with torch.cuda.device(dev):
-            _lib.check(lib.locus_hip_product_dev(args, torch.cuda.current_stream(dev).cuda_stream))
+            _lib.check(run_fn(args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _forward(fields, like):
+    lib = _lib.lib()
+    _run(_ARGS.pack, lib.locus_hip_product_workspace_bytes, lib.locus_hip_product_dev, fields, like)
 
 
 def _strides(t):
@@ -136,6 +139,21 @@ def _strides(t):
 
 def _ptr(t):
     return t.data_ptr() if t is not None else 0
+
+
+def _grouped_sizes(A, B, offsets, gather):
+    _operand("A", A, 2)
+    _operand("B", B, 3)
+    m, k = A.shape
+    groups, _, n = B.shape
+    _check("B", B, A, (groups, k, n))
+    if groups < 1:
+        _fail("B must hold at least one group")
+    _index("offsets", offsets, A, groups + 1)
+    if gather is not None:
+        _index("gather", gather, A, None)
+        m = gather.shape[0]
+    return m, n, k, groups
 
 
 def _outputs(A, m, n, out, pre, residual, reads):
@@ -171,10 +189,9 @@ def dense_product(A, B, bias=None, act="identity", residual=None, alpha=1.0, bet
     sbias = _bias_strides(bias, A, m, n) if bias is not None else (0, 0)
     out = _outputs(A, m, n, out, pre, residual, [("A", A), ("B", B), ("bias", bias)])
     if m and n:
-        _run(A.device.index, (m, n, k, _DTYPES[A.dtype], code, _DENSE, 0, *cfg, alpha, beta,
-                              A.data_ptr(), *A.stride(), B.data_ptr(), *B.stride(), _ptr(bias), *sbias,
-                              _ptr(residual), *_strides(residual), out.data_ptr(), *out.stride(),
-                              _ptr(pre), *_strides(pre), 0, 0, 0, 0, 0, 0, 0), A)
+        _forward((m, n, k, _DTYPES[A.dtype], code, _DENSE, 0, *cfg, alpha, beta, A.data_ptr(), *A.stride(),
+                  B.data_ptr(), *B.stride(), _ptr(bias), *sbias, _ptr(residual), *_strides(residual),
+                  out.data_ptr(), *out.stride(), _ptr(pre), *_strides(pre), 0, 0, 0, 0, 0, 0), A)
     return out
 
 
@@ -186,18 +203,7 @@ def grouped_product(A, B, offsets, bias=None, act="identity", residual=None, alp
     B (groups x k x n), bias (groups x n).  C has as many rows as `gather`, else as A; they are in the order of
     the runs (gathered rows are not moved back).  Runs may be empty.  Rows of no run are 0 in an `out` that
     is made here, and are left as they were in one that is given (and in its `pre`)."""
-    _operand("A", A, 2)
-    _operand("B", B, 3)
-    k = A.shape[1]
-    groups, _, n = B.shape
-    _check("B", B, A, (groups, k, n))
-    _index("offsets", offsets, A, groups + 1)
-    m = A.shape[0]
-    if gather is not None:
-        _index("gather", gather, A, None)
-        m = gather.shape[0]
-    if groups < 1:
-        _fail("B must hold at least one group")
+    m, n, k, groups = _grouped_sizes(A, B, offsets, gather)
     code = _act(act)
     if bias is not None:
         _check("bias", bias, A, (groups, n))
@@ -207,44 +213,39 @@ def grouped_product(A, B, offsets, bias=None, act="identity", residual=None, alp
     if m and n:
         sb = B.stride()
         sbias = bias.stride() if bias is not None else (0, 0)
-        _run(A.device.index, (m, n, k, _DTYPES[A.dtype], code, _ROWS, int(fill), *cfg, alpha, beta,
-                              A.data_ptr(), *A.stride(), B.data_ptr(), sb[1], sb[2], _ptr(bias), 0, sbias[1],
-                              _ptr(residual), *_strides(residual), out.data_ptr(), *out.stride(),
-                              _ptr(pre), *_strides(pre), groups, offsets.data_ptr(), sb[0], sbias[0], 0,
-                              _ptr(gather), A.shape[0]), A)
+        _forward((m, n, k, _DTYPES[A.dtype], code, _ROWS, int(fill), *cfg, alpha, beta, A.data_ptr(), *A.stride(),
+                  B.data_ptr(), sb[1], sb[2], _ptr(bias), 0, sbias[1], _ptr(residual), *_strides(residual),
+                  out.data_ptr(), *out.stride(), _ptr(pre), *_strides(pre), groups, offsets.data_ptr(), sb[0],
+                  sbias[0], _ptr(gather), A.shape[0]), A)
     return out
 
 
-def _slope(dC, pre, code, m, n, offsets, groups, col_sums, row_sums):
-    """G = dC act'(pre), with its column / row sums; dC itself for the identity."""
-    dev, dt = dC.device, _DTYPES[dC.dtype]
-    G = torch.empty((m, n), dtype=dC.dtype, device=dev) if code else None
-    if (G is None and col_sums is None and row_sums is None) or n == 0 or (m == 0 and col_sums is None):
-        return dC if G is None else G
-    lib = _lib.lib()
-    fields = (m, n, dt, code, dC.data_ptr(), *dC.stride(), _ptr(pre) if code else 0, *_strides(pre), _ptr(G),
-              _ptr(col_sums), _ptr(row_sums), groups, _ptr(offsets))
-    need = lib.locus_hip_product_slope_workspace_bytes(_SLOPE_ARGS.pack(*fields, 0, 0)) if col_sums is not None else 0
-    if need < 0:
-        _lib.check(int(need))
-    buf = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    args = _SLOPE_ARGS.pack(*fields, _ptr(buf), need)
-    with torch.cuda.device(dev):
-        _lib.check(lib.locus_hip_product_slope_dev(args, torch.cuda.current_stream(dev).cuda_stream))
-    return dC if G is None else G
-
-
-def _grad_inputs(dC, A, act, pre, m, n):
+def _gradient(dC, A, B, act, pre, alpha, need_A, need_B, bias_grad, m, n, k, groups, offsets, gather, cfg):
     code = _act(act)
     _check("dC", dC, A, (m, n))
     if code:
         if pre is None:
             _fail(f"the gradient of {act!r} needs pre, the Z kept by the forward call")
         _check("pre", pre, A, (m, n))
-    return code
+    new = lambda *shape: torch.empty(shape, dtype=A.dtype, device=A.device)  # noqa: E731
+    runs = (groups,) if groups else ()
+    dA = new(m, k) if need_A else None
+    dB = new(*runs, k, n) if need_B else None
+    db = {"column": lambda: new(*runs, n), "row": lambda: new(m, 1), "matrix": lambda: new(m, n) if code else dC.clone(),
+          None: lambda: None}[bias_grad]()
+    sb = B.stride()
+    lib = _lib.lib()
+    _run(_GRAD_ARGS.pack, lib.locus_hip_product_grad_workspace_bytes, lib.locus_hip_product_grad_dev,
+         (m, n, k, _DTYPES[A.dtype], code, _ROWS if groups else _DENSE, 0, *cfg, alpha, dC.data_ptr(), *dC.stride(),
+          _ptr(pre) if code else 0, *_strides(pre), A.data_ptr(), *A.stride(), B.data_ptr(), sb[-2], sb[-1],
+          _ptr(db) if bias_grad == "matrix" and code else 0, _ptr(dA), _ptr(dB), _ptr(db) if bias_grad == "column" else 0,
+          _ptr(db) if bias_grad == "row" else 0, groups, _ptr(offsets), sb[0] if groups else 0, _ptr(gather),
+          A.shape[0]), A)
+    return dA, dB, db
 
 
-def dense_product_grad(dC, A, B, act="identity", pre=None, alpha=1.0, need_A=True, need_B=True, bias_grad=None):
+def dense_product_grad(dC, A, B, act="identity", pre=None, alpha=1.0, need_A=True, need_B=True, bias_grad=None,
+                       cfg=(0, 0)):
     """(dA, dB, dbias) of dense_product from dC (m x n), with None for what is not asked for:
         G = dC act'(pre),  dA = alpha G B',  dB = alpha A' G,
     dbias = G summed to the shape of the bias: bias_grad = "column" (n,), "row" (m, 1), "matrix" (m, n) or
@@ -255,53 +256,18 @@ def dense_product_grad(dC, A, B, act="identity", pre=None, alpha=1.0, need_A=Tru
     m, k = A.shape
     n = B.shape[1]
     _check("B", B, A, (k, n))
-    code = _grad_inputs(dC, A, act, pre, m, n)
     if bias_grad not in (None, "column", "row", "matrix"):
         _fail(f"bias_grad must be None, 'column', 'row' or 'matrix', not {bias_grad!r}")
-    db = None
-    if bias_grad == "column":
-        db = torch.empty(n, dtype=A.dtype, device=A.device)
-    elif bias_grad == "row":
-        db = torch.zeros((m, 1), dtype=A.dtype, device=A.device) if n == 0 else \
-            torch.empty((m, 1), dtype=A.dtype, device=A.device)
-    G = _slope(dC, pre, code, m, n, None, 0, db if bias_grad == "column" else None,
-               db if bias_grad == "row" else None)
-    if bias_grad == "matrix":
-        db = G.clone() if G is dC else G
-    dA = dense_product(G, B.t(), alpha=alpha) if need_A else None
-    dB = dense_product(A.t(), G, alpha=alpha) if need_B else None
-    return dA, dB, db
+    return _gradient(dC, A, B, act, pre, alpha, need_A, need_B, bias_grad, m, n, k, 0, None, None, cfg)
 
 
 def grouped_product_grad(dC, A, B, offsets, act="identity", pre=None, alpha=1.0, gather=None, need_A=True,
-                         need_B=True, need_bias=False):
+                         need_B=True, need_bias=False, cfg=(0, 0)):
     """(dA, dB, dbias) of grouped_product, with None for what is not asked for:
         G[r] = dC[r] act'(pre[r]),  dA[r] = alpha G[r] B[g]',
         dB[g] = alpha sum_{r in g} A[src(r)]' G[r],  dbias[g] = sum_{r in g} G[r].
     dA has a row for each row of dC: with `gather` it is in the order of the runs, and the gradient of A's
     row i is the sum of the dA[r] with gather[r] = i.  Rows of no run: 0 in dA.  Empty runs: 0 in dB."""
-    _operand("A", A, 2)
-    _operand("B", B, 3)
-    k = A.shape[1]
-    groups, _, n = B.shape
-    _check("B", B, A, (groups, k, n))
-    _index("offsets", offsets, A, groups + 1)
-    m = A.shape[0]
-    if gather is not None:
-        _index("gather", gather, A, None)
-        m = gather.shape[0]
-    if groups < 1:
-        _fail("B must hold at least one group")
-    code = _grad_inputs(dC, A, act, pre, m, n)
-    db = torch.empty((groups, n), dtype=A.dtype, device=A.device) if need_bias else None
-    G = _slope(dC, pre, code, m, n, offsets, groups, db, None)
-    dA = grouped_product(G, B.transpose(1, 2), offsets, alpha=alpha) if need_A else None
-    dB = None
-    if need_B:
-        dB = torch.empty((groups, k, n), dtype=A.dtype, device=A.device)
-        if k and n:
-            _run(A.device.index, (k, n, m, _DTYPES[A.dtype], 0, _SUM, 0, 0, 0, alpha, 1.0,
-                                  A.data_ptr(), A.stride(1), A.stride(0), G.data_ptr(), *G.stride(), 0, 0, 0, 0, 0, 0,
-                                  dB.data_ptr(), n, 1, 0, 0, 0, groups, offsets.data_ptr(), 0, 0, k * n,
-                                  _ptr(gather), A.shape[0]), A)
-    return dA, dB, db
+    m, n, k, groups = _grouped_sizes(A, B, offsets, gather)
+    return _gradient(dC, A, B, act, pre, alpha, need_A, need_B, "column" if need_bias else None, m, n, k, groups, offsets,
+                     gather, cfg)

@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 
 DT = {"f64": torch.float64, "f32": torch.float32}
 ACTS = ("identity", "logistic", "probit", "softplus", "gelu", "silu")
-CFGS = [(0, 0), (1, 1), (1, 3), (2, 0), (4, 2), (64, 1), (64, 3), (128, 1), (128, 2)]
+CFGS = [(0, 0), (16, 1), (16, 3), (64, 1), (64, 3), (128, 1), (128, 2)]
 
 
 @pytest.fixture(scope="module")
@@ -139,7 +139,7 @@ def test_activation_values_and_slopes(pr, dtype, act):
     assert np.array_equal(host(g)[:, 0], limit)
 
 
-@pytest.mark.parametrize("cfg", [(1, 1), (4, 2), (64, 2), (128, 1)])
+@pytest.mark.parametrize("cfg", [(16, 1), (16, 2), (64, 2), (128, 1)])
 def test_nan_and_inf_stay_in_their_row_and_column(pr, cfg):
     rng = np.random.default_rng(5)
     m, k, n = 70, 45, 66
@@ -169,7 +169,7 @@ OFFSETS = {
 
 
 @pytest.mark.parametrize("dtype", ["f64", "f32"])
-@pytest.mark.parametrize("cfg", [(0, 0), (1, 1), (1, 3), (2, 0), (4, 2), (64, 1), (64, 2), (128, 1), (128, 3)])
+@pytest.mark.parametrize("cfg", [(0, 0), (16, 1), (16, 3), (64, 1), (64, 2), (128, 1), (128, 3)])
 @pytest.mark.parametrize("gather", [False, True])
 def test_grouped_product(pr, dtype, cfg, gather):
     t = DT[dtype]
@@ -205,7 +205,7 @@ def test_grouped_product(pr, dtype, cfg, gather):
             close(pre, zw, zt)
 
 
-@pytest.mark.parametrize("cfg", [(1, 1), (1, 2), (64, 1), (128, 2)])
+@pytest.mark.parametrize("cfg", [(16, 1), (16, 2), (64, 1), (128, 2)])
 def test_gathered_rows_outside_come_out_nan(pr, cfg):
     rng = np.random.default_rng(1)
     A, B = rng.normal(size=(9, 40)), rng.normal(size=(2, 40, 5))
@@ -238,9 +238,13 @@ def grad_reference(dC, A, B, act, pre, alpha, u):
     return G, tG, dA, tA, dB, tB, G.sum(axis=0), tb, (2 * (n + 4) * u * aG + tG).sum(axis=1, keepdims=True)
 
 
+GRAD_CFGS = [(0, 0), (16, 0), (64, 1), (64, 2), (128, 1), (128, 2)]
+
+
 @pytest.mark.parametrize("dtype", ["f64", "f32"])
 @pytest.mark.parametrize("act", ACTS)
-def test_dense_product_grad(pr, dtype, act):
+@pytest.mark.parametrize("cfg", GRAD_CFGS)
+def test_dense_product_grad(pr, dtype, act, cfg):
     t = DT[dtype]
     u = torch.finfo(t).eps / 2
     for i, (m, k, n) in enumerate([(1, 1, 1), (1, 50, 33), (67, 5, 20), (200, 130, 70), (700, 20, 3), (130, 33, 300)]):
@@ -250,7 +254,7 @@ def test_dense_product_grad(pr, dtype, act):
         G, tG, dA, tA, dB, tB, db, tb, tr = grad_reference(dC, A, B, act, pre, -0.5, u)
         lay = ("row", "col", "win")[i % 3]
         args = [layout(x, lay, t) for x in (dC, A, B)]
-        kw = dict(act=act, pre=layout(pre, lay, t), alpha=-0.5)
+        kw = dict(act=act, pre=layout(pre, lay, t), alpha=-0.5, cfg=cfg)
         ga, gb, gc = pr.dense_product_grad(*args, bias_grad="column", **kw)
         close(ga, dA, tA + 1e-300)
         close(gb, dB, tB + 1e-300)
@@ -266,7 +270,8 @@ def test_dense_product_grad(pr, dtype, act):
 @pytest.mark.parametrize("dtype", ["f64", "f32"])
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("name", list(OFFSETS))
-def test_grouped_product_grad(pr, dtype, gather, name):
+@pytest.mark.parametrize("cfg", GRAD_CFGS)
+def test_grouped_product_grad(pr, dtype, gather, name, cfg):
     t = DT[dtype]
     u = torch.finfo(t).eps / 2
     for j, (m, k, n) in enumerate([(1, 5, 3), (40, 33, 70), (600, 70, 65), (150, 140, 131)]):
@@ -289,7 +294,7 @@ def test_grouped_product_grad(pr, dtype, gather, name):
             tb[g] += r[7]
         got = pr.grouped_product_grad(dev(dC, t), layout(A, ("row", "col", "win", "row")[j], t), dev(B, t),
                                       torch.from_numpy(off).to("cuda:0"), act=act, pre=dev(pre, t), alpha=2.0,
-                                      gather=torch.from_numpy(src).to("cuda:0") if gather else None, need_bias=True)
+                                      gather=torch.from_numpy(src).to("cuda:0") if gather else None, need_bias=True, cfg=cfg)
         close(got[0], dA, tA)
         close(got[1], dB, tB)
         close(got[2], db, tb)
@@ -330,7 +335,7 @@ def test_gradients_against_differences(pr, act):
                 assert abs((fn(*up) - fn(*dn)) / (2 * h) - g[i]) < 1e-7
 
 
-@pytest.mark.parametrize("cfg", [(1, 1), (1, 2), (64, 1), (128, 2)])
+@pytest.mark.parametrize("cfg", [(16, 1), (16, 2), (64, 1), (128, 2)])
 def test_out_may_be_the_residual(pr, cfg):
     rng = np.random.default_rng(2)
     A, B, R = rng.normal(size=(70, 90)), rng.normal(size=(90, 66)), rng.normal(size=(70, 66))
@@ -353,7 +358,7 @@ def test_addresses_beyond_32_bits(pr, dtype):
     A.copy_(dev(rng.normal(size=(3, k)), t))
     B = dev(rng.normal(size=(k, n)), t)
     want = pr.dense_product(A.contiguous(), B)
-    for cfg in ((0, 0), (1, 2), (64, 1), (128, 2)):
+    for cfg in ((0, 0), (16, 2), (64, 1), (128, 2)):
         assert torch.equal(pr.dense_product(A, B, cfg=cfg), pr.dense_product(A.contiguous(), B, cfg=cfg))
         close(pr.dense_product(A, B, cfg=cfg), host(want), 2 * (k + 4) * unit(want) * (np.abs(host(A)) @ np.abs(host(B))))
     off = torch.tensor([0, 1, 4], device="cuda:0")
