@@ -129,13 +129,12 @@ __device__ __forceinline__ int bounded(int64_t v, int rows) { return v < 0 ? 0 :
 // 64 offsets at a time, one per lane: the ordered offsets are a running maximum, the tiles before a
 // run a running sum.  Every wave does this for itself (no barrier); under 1 us for up to 64 runs,
 // against a launch of its own for a tile map.  `tile` counts tiles of `bm` rows over all runs in
-// order; bm = 0 looks the run of row `tile` up instead.  first / last: the rows that runs cover.
-__device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int rows, int tile, int bm,
-                                        int* first = nullptr, int* last = nullptr)
+// order; bm = 0 looks the run of row `tile` up instead.  Where no run holds the tile: lo = the tiles there
+// are, hi = the end of the last run.
+__device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int rows, int tile, int bm)
 {
     const int lane = threadIdx.x & 63;
     int carry = bounded(offsets[0], rows);
-    if (first) *first = carry;
     int before = 0;                                    // tiles of the runs before this chunk
     Run found = {-1, 0, 0};
     for (int base = 0; base < groups; base += 64) {
@@ -166,18 +165,21 @@ __device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int 
             mine = tile >= lo && tile < hi;
         }
         const unsigned long long hit = __ballot(mine && g < groups);
-        if (hit && found.g < 0) {
+        if (hit) {
             const int src = __ffsll((long long)hit) - 1;
             found.g = base + src;
             const int rlo = __shfl(lo, src), rhi = __shfl(hi, src);
             const int t0 = bm ? rlo + (tile - __shfl(excl, src)) * bm : rlo;
             found.lo = t0;
             found.hi = bm && rhi - t0 > bm ? t0 + bm : rhi;
-            if (!last) break;
+            break;
         }
         carry = __shfl(hi, 63);
     }
-    if (last) *last = __builtin_amdgcn_readfirstlane(carry);
+    if (found.g < 0) {
+        found.lo = before;
+        found.hi = carry;
+    }
     found.g = __builtin_amdgcn_readfirstlane(found.g);
     found.lo = __builtin_amdgcn_readfirstlane(found.lo);
     found.hi = __builtin_amdgcn_readfirstlane(found.hi);
@@ -188,6 +190,7 @@ __device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int 
 __device__ __forceinline__ Run run_rows(const int64_t* offsets, int rows, int g)
 {
     const int lane = threadIdx.x & 63;
+    const int64_t last = offsets[g + 1];
     int top = 0;                                       // largest of offsets[0 .. g]
     for (int i = lane; i <= g; i += 64) {
         const int v = bounded(offsets[i], rows);
@@ -198,23 +201,23 @@ __device__ __forceinline__ Run run_rows(const int64_t* offsets, int rows, int g)
         const int o = __shfl_xor(top, s);
         top = o > top ? o : top;
     }
-    const int hi = bounded(offsets[g + 1], rows);
+    const int hi = bounded(last, rows);
     Run r = {g, __builtin_amdgcn_readfirstlane(top), 0};
     r.hi = __builtin_amdgcn_readfirstlane(hi > top ? hi : top);
     return r;
 }
 
-// Rows of no run become 0 (one workgroup per column block, of any size).
+// Rows of no run become 0: the workgroup behind the last tile takes the first bm of them, and so on.  There
+// are enough of those: the grid has m / bm + groups + 1 tiles, runs over all but R rows fill at most
+// (m - R) / bm + groups.  r: what find_run said of the tile.
 template <class T>
-__device__ __forceinline__ void fill_rest_rows(const ProductDesc& p, int n0, int n1)
+__device__ __forceinline__ void fill_rest_rows(const ProductDesc& p, const Run& r, int tile, int bm, int n0, int n1)
 {
-    int first, last;
-    find_run(p.offsets, p.groups, p.m, -1, 1, &first, &last);
-    const long outside = (long)first + (p.m - last);
-    const long w = n1 - n0;
-    for (long e = threadIdx.x; e < outside * w; e += blockDim.x) {
-        const long q = e / w, j = n0 + e % w;
-        const long i = q < first ? q : last + (q - first);
+    const int head = bounded(p.offsets[0], p.m), rest = head + (p.m - r.hi), w = n1 - n0;
+    const int q0 = (tile - r.lo) * bm, q1 = q0 + bm < rest ? q0 + bm : rest;
+    for (int e = threadIdx.x; e < (q1 - q0) * w; e += blockDim.x) {
+        const int q = q0 + e / w;
+        const long j = n0 + e % w, i = q < head ? q : r.hi + (q - head);
         static_cast<T*>(p.epi.C)[i * p.epi.sc_m + j * p.epi.sc_n] = T(0);
         if (p.epi.pre) static_cast<T*>(p.epi.pre)[i * p.epi.sp_m + j * p.epi.sp_n] = T(0);
     }

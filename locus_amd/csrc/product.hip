@@ -135,9 +135,10 @@ struct Want {
     long few;            // up to so many rows (or columns) take the kernel for few rows
 };
 
-// Which kernel, tile and split.  Times in microseconds from rates measured on this card (tiles: what a
-// CU reaches with one and with several workgroups on it; joining: the partials written and read at
-// 4.5 TB/s and one more launch).
+// Which kernel, tile and split.  A CU holds 4 workgroups of tiles of 64, 2 of 128; what share of its rate
+// it reaches with 1, 2, .. of them was measured (2000 x 500 x 20 000, both types within 3 %), as were the
+// microseconds a round of workgroups takes beside its products, and a joining launch: its own and the
+// partials written and read at 4.5 TB/s.
 Plan plan_product(const Want& w)
 {
     Plan pl;
@@ -179,9 +180,13 @@ Plan plan_product(const Want& w)
             const long chunk = ((K + nz - 1) / nz + bk - 1) / bk * bk;
             if (!w.cfg[1] && nz > 1 && chunk < 8 * bk) break;
             const long used = K > 0 ? (K + chunk - 1) / chunk : 1;
-            const long wgs = tiles * used, load = (wgs + w.cus - 1) / w.cus;
-            const double eff = tw == 4 ? (load == 1 ? 0.7 : 0.92) : (load == 1 ? 0.6 : (load == 2 ? 0.75 : 0.87));
-            double t = load * 2.0 * bm * bm * chunk / (cu_rate * eff);
+            const long wgs = tiles * used, load = (wgs + w.cus - 1) / w.cus, slots = tw == 4 ? 2 : 4;
+            static const double share2[5] = {0, 0.67, 0.80, 0.86, 0.90}, share4[3] = {0, 0.86, 0.92};
+            const double* share = tw == 4 ? share4 : share2;
+            const double one = 2.0 * bm * bm * chunk / cu_rate;          // a workgroup's products on its CU
+            const long rest = load % slots;
+            double t = one * ((load - rest) / share[slots] + (rest ? rest / share[rest] : 0.0)) +
+                       (double)((load + slots - 1) / slots) * (tw == 4 ? 9.0 : 6.0);
             if (used > 1) t += 4.0 + 2.0 * used * M * N * s / 4.5e6;
             if (t < best) {
                 best = t;
@@ -306,12 +311,12 @@ Want want_product(const locus_hip_product_args& a)
 // ---- gradient ------------------------------------------------------------------------------------
 
 // Parts of a run whose column sums are taken side by side: about two workgroups (of 16 waves) per CU,
-// parts of at least 64 rows.
+// parts of at least 256 rows (fewer are as quick as the launch that would join them).
 int slope_parts(const locus_hip_product_grad_args& a)
 {
     const long blocks = ((a.n + 63) / 64) * std::max<long>(1, a.groups);
     const long per = a.m / std::max<long>(1, a.groups);
-    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks), per / 64);
+    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks), per / 256);
     return (int)std::max<long>(1, std::min<long>(want, 1024));
 }
 
@@ -379,8 +384,15 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     q.epi.C = a.dB; q.epi.sc_m = a.n; q.epi.sc_n = 1;
     q.sc_g = a.k * a.n;
     if (runs) { q.gather = a.gather; q.a_rows = a.a_rows; }
-    if (a.dA) { r.pa = plan_product(r.da); r.a_bytes = up(plan_bytes(r.da, r.pa)); }
-    if (a.dB) { r.pb = plan_product(r.db); r.b_bytes = up(plan_bytes(r.db, r.pb)); }
+    if (a.dA) r.pa = plan_product(r.da);
+    if (a.dB) r.pb = plan_product(r.db);
+    if (a.dA && a.dB && !r.pa.rows && !r.pb.rows && r.pa.tw != r.pb.tw) {   // one launch wants one tile
+        r.da.cfg[0] = r.db.cfg[0] = 64;
+        r.pa = plan_product(r.da);
+        r.pb = plan_product(r.db);
+    }
+    if (a.dA) r.a_bytes = up(plan_bytes(r.da, r.pa));
+    if (a.dB) r.b_bytes = up(plan_bytes(r.db, r.pb));
     return r;
 }
 

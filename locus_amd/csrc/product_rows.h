@@ -60,12 +60,11 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
         m0 = (long)tile * BM;
         mEnd = p.m;
     } else {
-        if (p.fill_rest && tile == gridDim.x - 1) {
-            if (blockIdx.z == 0) fill_rest_rows<T>(p, n0, n0 + 64 < p.n ? n0 + 64 : p.n);
+        const Run r = find_run(p.offsets, p.groups, p.m, tile, BM);
+        if (r.g < 0) {
+            if (p.fill_rest && blockIdx.z == 0) fill_rest_rows<T>(p, r, tile, BM, n0, n0 + 64 < p.n ? n0 + 64 : p.n);
             return;
         }
-        const Run r = find_run(p.offsets, p.groups, p.m, tile, BM);
-        if (r.g < 0) return;
         m0 = r.lo;
         mEnd = r.hi;
         B += r.g * p.sb_g;

@@ -196,10 +196,15 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
         const unsigned w = xcd * (total >> 3) + (xcd < rem ? xcd : rem) + (lin >> 3);
         bz = w / each;
         const unsigned t = w - bz * each;
-        const unsigned panel = t / (8 * gy), r = t - panel * 8 * gy;
-        const unsigned high = gx - panel * 8 < 8 ? gx - panel * 8 : 8;
-        by = r / high;
-        bx = panel * 8 + r - by * high;
+        if (MODE == PRODUCT_ROWS) {     // tiles of no run lie at the end of every column: each XCD gets its share
+            by = t / gx;
+            bx = t - by * gx;
+        } else {
+            const unsigned panel = t / (8 * gy), r = t - panel * 8 * gy;
+            const unsigned high = gx - panel * 8 < 8 ? gx - panel * 8 : 8;
+            by = r / high;
+            bx = panel * 8 + r - by * high;
+        }
     }
     const int n0 = by * BN, nEnd = p.n;
     long m0, mEnd;                      // rows of C
@@ -211,12 +216,11 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
         m0 = (long)bx * BM;
         mEnd = p.m;
     } else if constexpr (MODE == PRODUCT_ROWS) {
-        if (p.fill_rest && bx == gx - 1) {
-            if (bz == 0) fill_rest_rows<T>(p, n0, n0 + BN < p.n ? n0 + BN : p.n);
+        const Run r = find_run(p.offsets, p.groups, p.m, bx, BM);
+        if (r.g < 0) {
+            if (p.fill_rest && bz == 0) fill_rest_rows<T>(p, r, bx, BM, n0, n0 + BN < p.n ? n0 + BN : p.n);
             return;
         }
-        const Run r = find_run(p.offsets, p.groups, p.m, bx, BM);
-        if (r.g < 0) return;
         m0 = r.lo;
         mEnd = r.hi;
         B += r.g * p.sb_g;
@@ -319,8 +323,8 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
         Ab += da;
         Bb += db;
     };
-    auto write_part = [&](auto bufc, int q0, int q1) {
-        constexpr int buf = decltype(bufc)::value, st = buf % PF;
+    auto write_part = [&](auto tc, int q0, int q1) {
+        constexpr int buf = decltype(tc)::value, st = buf % PF;
 #pragma unroll
         for (int q = q0; q < q1; ++q) {
             al[buf * BUF + q * aq] = ra[st][q];
@@ -345,9 +349,8 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
     // wave's matrix instructions never wait for an LDS read just issued; tile t + 1 goes to LDS and
     // tile t + 1 + PF is requested in pieces between them.  CHECK: the last tiles, which ask what is left.
     auto k_tile = [&](auto bufc, auto checkc, int t) {
-        constexpr int buf = decltype(bufc)::value;
         constexpr bool CHECK = decltype(checkc)::value;
-        constexpr auto nextc = std::integral_constant<int, buf ^ 1>{};
+        constexpr auto nextc = std::integral_constant<int, (decltype(bufc)::value ^ 1)>{};
         const bool more = !CHECK || t + 1 < tiles;
         const int kl = kb + (t + 1 + PF) * BK;
         const bool ask = !CHECK || t + 1 + PF < tiles;
