@@ -46,6 +46,8 @@ extern "C" {
                                        points of section 1 return without touching the caller's
                                        buffers.  The reference's sweep cannot fail half-way
                                        (src/coreLoop.cpp:36-52).  Serialise cluster sweeps per GPU. */
+#define LOCUS_HIP_EWORKSPACE (-5)   /* locus_hip_product_*: no workspace, or one too small; nothing was
+                                       launched                                                  */
 
 const char* locus_hip_last_error(void);
 int locus_hip_version(void);      /* 100 * major + minor */
@@ -313,8 +315,10 @@ typedef struct locus_hip_product_args {
     const void* B; int64_t sb_k, sb_n;
     const void* bias; int64_t sbias_m, sbias_n;   /* or NULL; a stride of 0 broadcasts          */
     const void* res; int64_t sr_m, sr_n;          /* or NULL; may be C (same strides)           */
-    void* C; int64_t sc_m, sc_n;
-    void* pre; int64_t sp_m, sp_n;                /* or NULL: receives Z; not C                 */
+    void* C; int64_t sc_m, sc_n;                  /* C and pre: rows (or columns) one behind the
+                                                     other, sharing no memory with each other or
+                                                     with what is read (else LOCUS_HIP_EINVAL)   */
+    void* pre; int64_t sp_m, sp_n;                /* or NULL: receives Z                        */
     int64_t groups; const int64_t* offsets;       /* [groups + 1]                               */
     int64_t sb_g, sbias_g;
     const int64_t* gather; int64_t a_rows;        /* [m] or NULL                                */

@@ -124,6 +124,13 @@ struct Run {
     int lo, hi;       // its rows (of the tile asked for)
 };
 
+__device__ __forceinline__ long uniform_long(long v)
+{
+    const int lo = __builtin_amdgcn_readfirstlane((int)(v & 0xffffffff));
+    const int hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return ((long)hi << 32) | (unsigned)lo;
+}
+
 __device__ __forceinline__ int bounded(int64_t v, int rows) { return v < 0 ? 0 : (v > rows ? rows : (int)v); }
 
 // 64 offsets at a time, one per lane: the ordered offsets are a running maximum, the tiles before a
@@ -207,9 +214,44 @@ __device__ __forceinline__ Run run_rows(const int64_t* offsets, int rows, int g)
     return r;
 }
 
+// The run of each lane's own row (-1: none): the same scan, then every run of the 64 offered to all lanes.
+__device__ __forceinline__ int find_runs(const int64_t* offsets, int groups, int rows, int row)
+{
+    const int lane = threadIdx.x & 63;
+    int carry = bounded(offsets[0], rows), found = -1;
+    for (int base = 0; base < groups; base += 64) {
+        const int g = base + lane;
+        int hi = g < groups ? bounded(offsets[g + 1], rows) : 0;
+        hi = hi > carry ? hi : carry;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int o = __shfl_up(hi, s);
+            if (lane >= s && o > hi) hi = o;
+        }
+        const int here = groups - base < 64 ? groups - base : 64;
+        int lo = carry;
+        for (int s = 0; s < here; ++s) {
+            const int top = __builtin_amdgcn_readlane(hi, s);
+            if (row >= lo && row < top) found = base + s;
+            lo = top;
+        }
+        carry = lo;
+        if (__ballot(row >= carry) == 0) break;
+    }
+    return found;
+}
+
+// Tiles of bm rows that runs can have at most: full ones and one partial tile per run, none without a row;
+// and one more, so that the tiles behind the last one cover the rows of no run (fill_rest_rows).
+inline unsigned run_tiles(const ProductDesc& p, int bm)
+{
+    const long most = (long)p.m / bm + p.groups;
+    return (unsigned)((most < p.m ? most : p.m) + (p.fill_rest ? 1 : 0));
+}
+
 // Rows of no run become 0: the workgroup behind the last tile takes the first bm of them, and so on.  There
-// are enough of those: the grid has m / bm + groups + 1 tiles, runs over all but R rows fill at most
-// (m - R) / bm + groups.  r: what find_run said of the tile.
+// are enough of those: the grid has min(m / bm + groups, m) + 1 tiles, runs over all but R rows fill at
+// most (m - R) / bm + groups and at most m - R of them.  r: what find_run said of the tile.
 template <class T>
 __device__ __forceinline__ void fill_rest_rows(const ProductDesc& p, const Run& r, int tile, int bm, int n0, int n1)
 {

@@ -2,6 +2,8 @@
 // (joining a split sum, the gradient before the activation, column and row sums) and the C entry
 // points locus_hip_product_* (include/locus_hip.h).
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 #include "product.h"
 
@@ -10,8 +12,8 @@ namespace locus {
 namespace {
 
 // C from the partial products of a split sum, added in the order of the slices (the same result
-// every time).  Bound by reading them; DENSE: one thread per element along the partials' contiguous index;
-// ROWS: a workgroup per row, which looks its run up for the bias.
+// every time).  Bound by reading them; one thread per element along the partials' contiguous index; in
+// ROWS a lane looks its row's run up for the bias.
 template <class T, int MODE>
 __global__ void __launch_bounds__(256) product_join_kernel(const ProductDesc p)
 {
@@ -22,17 +24,16 @@ __global__ void __launch_bounds__(256) product_join_kernel(const ProductDesc p)
         for (int z = 0; z < p.nz; ++z) v += x[z * p.part_z];
         epi_store<T>(p.epi, bias0, i, j, v);
     };
-    if constexpr (MODE == PRODUCT_DENSE) {
-        const long len = (long)p.m * p.n;
-        for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < len; e += (long)gridDim.x * 256) {
+    const long len = (long)p.m * p.n;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < (len + 63) / 64 * 64; e += (long)gridDim.x * 256) {
+        if constexpr (MODE == PRODUCT_DENSE) {
+            if (e >= len) break;
             if (p.part_m == 1) join(0, e % p.m, e / p.m);
             else join(0, e / p.n, e % p.n);
-        }
-    } else {
-        const long j = (long)blockIdx.y * 256 + threadIdx.x;
-        for (long i = blockIdx.x; i < p.m; i += gridDim.x) {
-            const Run r = find_run(p.offsets, p.groups, p.m, i, 0);
-            if (r.g >= 0 && j < p.n) join(r.g * p.sbias_g, i, j);
+        } else {                                          // whole waves stay together for the lookup
+            const long i = e < len ? e / p.n : p.m - 1;
+            const int g = find_runs(p.offsets, p.groups, p.m, (int)i);
+            if (g >= 0 && e < len) join(g * p.sbias_g, i, e % p.n);
         }
     }
 }
@@ -132,7 +133,8 @@ struct Want {
     bool f64;
     int cfg[2];
     long cus;            // CUs it may count on
-    long few;            // up to so many rows (or columns) take the kernel for few rows
+    long few, large;     // up to so many rows (or columns) take the kernel for few rows, where the other
+                         // factor has so many elements
 };
 
 // Which kernel, tile and split.  A CU holds 4 workgroups of tiles of 64, 2 of 128; what share of its rate
@@ -153,15 +155,15 @@ Plan plan_product(const Want& w)
         return pl;
     }
     const long side = runs ? (long)avg : std::min(M, N);
-    pl.rows = w.cfg[0] ? w.cfg[0] == 16 : side <= w.few;
+    pl.rows = w.cfg[0] ? w.cfg[0] == 16 : side <= w.few && (runs || std::max(M, N) * K >= w.large);
     if (pl.rows) {
         pl.swap = !runs && N < M;
         const long m = pl.swap ? N : M, n = pl.swap ? M : N, kb = w.f64 ? 8 : 16;
         const long rt = runs ? std::max<long>(1, std::min<long>(m, m / 16 + p.groups)) : (m + 15) / 16;
         const long wgs = rt * ((n + 63) / 64);
-        // two workgroups a CU; a wave gets 16 blocks of k at least (a launch to join costs as much), and the
-        // partials stay within a tenth of B
-        long nz = std::min<long>(2 * w.cus / wgs, K / (64 * kb));
+        // two workgroups a CU; a sum that one workgroup ends in 24 blocks of k a wave is not split (a launch to
+        // join costs as much), else a wave gets 8 at least, and the partials stay within a tenth of B
+        long nz = std::min<long>(2 * w.cus / wgs, K > 96 * kb ? K / (32 * kb) : 1);
         nz = std::min<long>(nz, (long)(0.1 * K / (runs ? avg : (double)m)));
         if (w.cfg[1]) nz = w.cfg[1];
         nz = std::max<long>(1, std::min<long>(nz, 256));
@@ -170,6 +172,9 @@ Plan plan_product(const Want& w)
         return pl;
     }
     const double cu_rate = (w.f64 ? 75e6 : 150e6) / w.cus;     // flop per us
+    // us a workgroup alone on its CU takes for a million elements of the activation
+    const bool cdf = p.epi.act == LOCUS_HIP_ACT_PROBIT || p.epi.act == LOCUS_HIP_ACT_GELU;
+    const double heavy = p.epi.act == LOCUS_HIP_ACT_IDENTITY ? 0.0 : (w.f64 ? (cdf ? 2200.0 : 1000.0) : 400.0);
     double best = 1e300;
     for (int tw = 4; tw >= 2; tw -= 2) {
         if (w.cfg[0] && w.cfg[0] != 32 * tw) continue;
@@ -178,7 +183,7 @@ Plan plan_product(const Want& w)
         const long tiles = std::max<long>(mt, 1) * ((N + bm - 1) / bm);
         for (long nz = w.cfg[1] ? w.cfg[1] : 1; nz <= (w.cfg[1] ? w.cfg[1] : 32); ++nz) {
             const long chunk = ((K + nz - 1) / nz + bk - 1) / bk * bk;
-            if (!w.cfg[1] && nz > 1 && chunk < 8 * bk) break;
+            if (!w.cfg[1] && nz > 1 && chunk < 4 * bk) break;
             const long used = K > 0 ? (K + chunk - 1) / chunk : 1;
             const long wgs = tiles * used, load = (wgs + w.cus - 1) / w.cus, slots = tw == 4 ? 2 : 4;
             static const double share2[5] = {0, 0.67, 0.80, 0.86, 0.90}, share4[3] = {0, 0.86, 0.92};
@@ -187,6 +192,9 @@ Plan plan_product(const Want& w)
             const long rest = load % slots;
             double t = one * ((load - rest) / share[slots] + (rest ? rest / share[rest] : 0.0)) +
                        (double)((load + slots - 1) / slots) * (tw == 4 ? 9.0 : 6.0);
+            // the element function: in the epilogue by a CU's workgroups, after a split by all CUs
+            const double f = 1e-6 * bm * bm * heavy;
+            t += used == 1 ? f * std::max<double>(1.0, (double)wgs / w.cus / 2) : f * tiles / w.cus / 2;
             if (used > 1) t += 4.0 + 2.0 * used * M * N * s / 4.5e6;
             if (t < best) {
                 best = t;
@@ -235,12 +243,9 @@ ProductDesc planned(const Want& w, const Plan& pl, void* part)
 template <class T> int join_product(const ProductDesc& p, int mode, hipStream_t st)
 {
     if (p.nz <= 1) return 0;
-    if (mode == PRODUCT_DENSE)
-        hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_DENSE>), dim3(grid_of(((long)p.m * p.n + 255) / 256)),
-                           dim3(256), 0, st, p);
-    else
-        hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_ROWS>), dim3(grid_of(p.m), (unsigned)((p.n + 255) / 256)),
-                           dim3(256), 0, st, p);
+    const dim3 grid(grid_of(((long)p.m * p.n + 255) / 256));
+    if (mode == PRODUCT_DENSE) hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_DENSE>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_ROWS>), grid, dim3(256), 0, st, p);
     LOCUS_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -268,15 +273,71 @@ int check_common(const char* what, int64_t m, int64_t n, int64_t k, int dtype, i
                   w + ": the kernel for few rows takes fewer than 2^20 of them");
     if (mode == LOCUS_HIP_PRODUCT_ROWS) {
         LOCUS_REQUIRE(groups >= 1 && groups <= 65535, w + ": groups (1..65535)");
-        LOCUS_REQUIRE(!gather || a_rows >= 0, w + ": a_rows");
+        LOCUS_REQUIRE(!gather || (a_rows >= 0 && a_rows < (1ll << 31)), w + ": a_rows");
     }
     return 0;
+}
+
+int no_workspace(const char* fn)
+{
+    set_error(std::string("workspace smaller than ") + fn);
+    return LOCUS_HIP_EWORKSPACE;
 }
 
 int check_product(const locus_hip_product_args* a)
 {
     LOCUS_REQUIRE(a, "product: no arguments");
     return check_common("product", a->m, a->n, a->k, a->dtype, a->act, a->mode, a->cfg, a->groups, a->gather, a->a_rows);
+}
+
+// The bytes that a strided array spans.
+struct Span {
+    const char *lo = nullptr, *hi = nullptr;
+    Span(const void* at, long size, std::initializer_list<std::pair<long, long>> dims)
+    {
+        if (!at) return;
+        long back = 0, ahead = 0;
+        for (auto [n, s] : dims) {
+            if (n == 0) return;
+            (s < 0 ? back : ahead) += (n - 1) * s;
+        }
+        lo = static_cast<const char*>(at) + back * size;
+        hi = static_cast<const char*>(at) + (ahead + 1) * size;
+    }
+    bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+
+// Rows (or columns) that lie one behind the other: every element has memory of its own.
+bool apart(long m, long sm, long n, long sn)
+{
+    sm = sm < 0 ? -sm : sm;
+    sn = sn < 0 ? -sn : sn;
+    if (m == 1) return n == 1 || sn >= 1;
+    if (n == 1) return sm >= 1;
+    return sm <= sn ? sm >= 1 && sn > sm * (m - 1) : sn >= 1 && sm > sn * (n - 1);
+}
+
+int check_spans(const locus_hip_product_args& a)
+{
+    const long s = a.dtype == LOCUS_HIP_F64 ? 8 : 4;
+    const bool runs = a.mode == LOCUS_HIP_PRODUCT_ROWS;
+    const long groups = runs ? a.groups : 1;
+    const Span C(a.C, s, {{a.m, a.sc_m}, {a.n, a.sc_n}}), pre(a.pre, s, {{a.m, a.sp_m}, {a.n, a.sp_n}});
+    const Span res(a.res, s, {{a.m, a.sr_m}, {a.n, a.sr_n}});
+    const Span reads[] = {Span(a.A, s, {{runs && a.gather ? a.a_rows : a.m, a.sa_m}, {a.k, a.sa_k}}),
+                          Span(a.B, s, {{groups, a.sb_g}, {a.k, a.sb_k}, {a.n, a.sb_n}}),
+                          Span(a.bias, s, {{groups, a.sbias_g}, {a.m, a.sbias_m}, {a.n, a.sbias_n}}),
+                          Span(runs ? a.offsets : nullptr, 8, {{groups + 1, 1}}),
+                          Span(runs ? a.gather : nullptr, 8, {{a.m, 1}})};
+    LOCUS_REQUIRE(apart(a.m, a.sc_m, a.n, a.sc_n), "product: elements of C share memory");
+    LOCUS_REQUIRE(!a.pre || apart(a.m, a.sp_m, a.n, a.sp_n), "product: elements of pre share memory");
+    for (const Span& r : reads)
+        LOCUS_REQUIRE(!C.meets(r) && !pre.meets(r), "product: C or pre shares memory with what is read");
+    LOCUS_REQUIRE(!C.meets(pre), "product: C shares memory with pre");
+    LOCUS_REQUIRE(!pre.meets(res), "product: pre shares memory with the residual");
+    LOCUS_REQUIRE(!C.meets(res) || (a.C == a.res && a.sc_m == a.sr_m && a.sc_n == a.sr_n),
+                  "product: C shares memory with the residual and is not it");
+    return 0;
 }
 
 Want want_product(const locus_hip_product_args& a)
@@ -310,13 +371,15 @@ Want want_product(const locus_hip_product_args& a)
 
 // ---- gradient ------------------------------------------------------------------------------------
 
-// Parts of a run whose column sums are taken side by side: about two workgroups (of 16 waves) per CU,
-// parts of at least 256 rows (fewer are as quick as the launch that would join them).
+// Parts of a run whose G and column sums are taken side by side: about two workgroups (of 16 waves) per
+// CU.  A part has rows enough to be worth the launch that joins them: 16 waves do 256 rows without an
+// activation, 64 with one (a 16-row turn of a float64 slope takes 2 to 3 us on a CU) in its time.
 int slope_parts(const locus_hip_product_grad_args& a)
 {
     const long blocks = ((a.n + 63) / 64) * std::max<long>(1, a.groups);
     const long per = a.m / std::max<long>(1, a.groups);
-    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks), per / 256);
+    const long least = a.act == LOCUS_HIP_ACT_IDENTITY ? 256 : 64;
+    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks), per / least);
     return (int)std::max<long>(1, std::min<long>(want, 1024));
 }
 
@@ -360,6 +423,7 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     w.cfg[0] = a.cfg[0]; w.cfg[1] = a.cfg[1];
     w.cus = a.dA && a.dB ? device_cus() / 2 : device_cus();
     w.few = 16;
+    w.large = 1 << 19;   // below, the two products in one launch are quicker
     w.p.epi.alpha = a.alpha;
     if (runs) {
         w.p.groups = (int)a.groups;
@@ -462,12 +526,12 @@ int locus_hip_product_dev(const locus_hip_product_args* args, void* stream)
     if (a.m == 0 || a.n == 0) return 0;
     LOCUS_REQUIRE(a.C && (a.k == 0 || (a.A && a.B)), "product: null pointer");
     LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || a.offsets, "product: runs need offsets");
-    LOCUS_REQUIRE(a.pre != a.C, "product: pre and C are two buffers");
-    LOCUS_REQUIRE(!a.gather || a.a_rows > 0 || a.k == 0, "product: rows gathered from an empty matrix");
+    LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || !a.gather || a.a_rows > 0 || a.k == 0,
+                  "product: rows gathered from an empty matrix");
+    if ((rc = check_spans(a))) return rc;
     const Want w = want_product(a);
     const Plan pl = plan_product(w);
-    LOCUS_REQUIRE(plan_bytes(w, pl) <= (a.workspace ? a.workspace_bytes : 0),
-                  "product: workspace smaller than locus_hip_product_workspace_bytes()");
+    if (plan_bytes(w, pl) > (a.workspace ? a.workspace_bytes : 0)) return no_workspace("locus_hip_product_workspace_bytes()");
     return w.f64 ? run_product<double>(w, pl, a.workspace, (hipStream_t)stream)
                  : run_product<float>(w, pl, a.workspace, (hipStream_t)stream);
 }
@@ -488,10 +552,10 @@ int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* st
     LOCUS_REQUIRE(!a.dA || a.B || a.k == 0 || a.n == 0 || a.m == 0, "product_grad: dA needs B");
     LOCUS_REQUIRE(!a.dB || a.A || a.k == 0 || a.n == 0 || a.m == 0, "product_grad: dB needs A");
     LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || a.offsets, "product_grad: runs need offsets");
-    LOCUS_REQUIRE(!a.gather || a.a_rows > 0 || a.m == 0 || a.k == 0, "product_grad: rows gathered from an empty matrix");
+    LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || !a.gather || a.a_rows > 0 || a.m == 0 || a.k == 0,
+                  "product_grad: rows gathered from an empty matrix");
     Grad r = plan_grad(a);
-    LOCUS_REQUIRE(r.all() <= (a.workspace ? a.workspace_bytes : 0),
-                  "product_grad: workspace smaller than locus_hip_product_grad_workspace_bytes()");
+    if (r.all() > (a.workspace ? a.workspace_bytes : 0)) return no_workspace("locus_hip_product_grad_workspace_bytes()");
     return a.dtype == LOCUS_HIP_F64 ? run_grad<double>(a, r, (hipStream_t)stream) : run_grad<float>(a, r, (hipStream_t)stream);
 }
 

@@ -237,7 +237,7 @@ int launch_product_rows(const ProductDesc& p, int mode, hipStream_t st)
     constexpr int V = Vec16<T>::V;
     const unsigned gx = (unsigned)((p.n + 63) / 64);
     const unsigned gy = mode == PRODUCT_DENSE ? (unsigned)((p.m + 15) / 16)
-                                              : (unsigned)(p.m / 16 + p.groups + (p.fill_rest ? 1 : 0));
+                                              : run_tiles(p, 16);
     const int kind = p.sb_n == 1 && p.n >= V ? ROWS_BK_N : (p.sb_k == 1 ? ROWS_BK_K : ROWS_BK_ANY);
     const bool dense = mode == PRODUCT_DENSE;
     auto pick = [&](auto kc) {

@@ -171,7 +171,7 @@ __device__ __forceinline__ void store_block(const ProductDesc& p, const T* lds, 
 
 // How a kernel is compiled for the operands: FAST with each operand's contiguous index (k or not),
 // or the general form: run-time layouts and 64-bit lane addresses.
-enum { LAY_ANY = 0, LAY_FAST = 1, LAY_A_K = 2, LAY_B_K = 4 };
+enum { LAY_ANY = 0, LAY_FAST = 1, LAY_A_K = 2, LAY_B_K = 4, LAY_GATHER = 8 /* a fast sum's gathered A */ };
 
 // Workgroup `lin` of a grid of gx x gy x gz.
 template <class T, int TW, int BK, int PF, int MODE, int LAY>
@@ -229,9 +229,21 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
         const Run r = run_rows(p.offsets, p.k, bz);
         m0 = (long)bx * BM;
         mEnd = p.m;
-        kb = (int)r.lo;
-        kEnd = (int)r.hi;
+        kb = r.lo;
+        kEnd = r.hi;
         c0 = r.g * p.sc_g;
+        if (kb >= kEnd) {               // an empty run: 0
+            const int w = nEnd - n0 < BN ? nEnd - n0 : BN;
+            T* C = static_cast<T*>(p.epi.C) + c0 + m0 * p.epi.sc_m + n0;
+            const int h = (int)(mEnd - m0 < BM ? mEnd - m0 : BM);
+            if (w == p.epi.sc_m) {      // whole rows: one piece of memory
+                for (int e = tid; e < h * w; e += 256) C[e] = T(0);
+            } else {
+                for (int i = tid / BN; i < h; i += 256 / BN)
+                    if (tid % BN < w) C[i * p.epi.sc_m + tid % BN] = T(0);
+            }
+            return;
+        }
     }
     if constexpr (MODE != PRODUCT_SUM) {
         if (p.part) {
@@ -255,14 +267,18 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
 
     // Row of A behind row i of the tile; gathered indexes outside A count as 0 here (they never reach
     // a result: the epilogue makes it NaN).  Base: the tile's first row, gathered: A's first.
-    const bool gr = MODE == PRODUCT_ROWS && p.gather, gs = MODE == PRODUCT_SUM && p.gather;
+    const bool gr = MODE == PRODUCT_ROWS && p.gather;
+    const bool gs = MODE == PRODUCT_SUM && (FAST ? (LAY & LAY_GATHER) != 0 : p.gather != nullptr);
     auto in_a = [&](long row) { return row >= 0 && row < p.a_rows ? row : 0; };
     auto a_row = [&](int i) -> long {
         const int c = i < mRows ? i : 0;
         return gr ? in_a(p.gather[m0 + c]) : c;
     };
-    const char* Ab = reinterpret_cast<const char*>(A + (gr ? 0 : m0 * p.sa_m) + (gs ? 0 : kb * p.sa_k));
-    const char* Bb = reinterpret_cast<const char*>(B + (long)n0 * p.sb_n + kb * p.sb_k);
+    // (readfirstlane: the compiler does not see that a run's base is the same for all lanes, and would
+    // ask lane by lane for each load of the K loop)
+    auto base = [&](const T* at) { return reinterpret_cast<const char*>(uniform_long(reinterpret_cast<long>(at))); };
+    const char* Ab = base(A + (gr ? 0 : m0 * p.sa_m) + (gs ? 0 : kb * p.sa_k));
+    const char* Bb = base(B + (long)n0 * p.sb_n + kb * p.sb_k);
     const long da = (gs ? 0 : BK * p.sa_k) * sz, db = BK * p.sb_k * sz;
     // Lane offsets in bytes: one per element where k is contiguous (rows are clamped one by one), else one, and
     // the step of q on the scalar unit.
@@ -289,14 +305,18 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
     T ra[PF][NQ], rb[PF][NQ];           // [stage]: K-tiles on their way
     // Element q of the K-tile that starts at k0; `in`: k is not beyond the end.  An element beyond it is 0: FAST
     // asks for an offset outside the buffer resource, which the hardware answers with 0 (no branches in
-    // short sums).  Gathered sums: one row of A per wave and element.
-    auto get_a = [&](int q, int k0, bool in) -> T {
+    // short sums).  Gathered sums: one row of A per wave and element; lane q holds the q-th one of the
+    // K-tile (rows), read a K-tile ahead.
+    auto gathered = [&](int k0) -> int {
+        if (MODE != PRODUCT_SUM || !gs) return 0;
+        const int k = k0 + ak0 + lane % NQ * QM;
+        return (int)in_a(p.gather[k < kEnd ? k : kb]);
+    };
+    auto get_a = [&](int q, int rows, bool in) -> T {
         if (MODE == PRODUCT_SUM && gs) {
-            if constexpr (!FAST) if (!in) return T(0);
-            const int k = k0 + ak0 + q * QM;                    // the same for a whole wave
-            const long row = in_a(p.gather[in ? k : kb]) * p.sa_k * sz;
+            const long row = (long)__builtin_amdgcn_readlane(rows, q) * p.sa_k * sz;
             if constexpr (FAST) return buffer_elem<T>(Ab, in ? oa[0] : 0x80000000u, (unsigned)row);
-            else return *reinterpret_cast<const T*>(Ab + row + oa[q]);
+            else return in ? *reinterpret_cast<const T*>(Ab + row + oa[q]) : T(0);
         }
         if constexpr (FAST)
             return buffer_elem<T>(Ab, in ? oa[AKF ? q : 0] : 0x80000000u, AKF ? 0u : (unsigned)(q * QM * p.sa_k * sz));
@@ -310,15 +330,16 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
             return in ? *reinterpret_cast<const T*>(Bb + ob[q]) : T(0);
     };
     // The K-tile whose first k is k0, elements [q0, q1) of each operand, to registers (stage st).
-    auto load_part = [&](auto stc, auto wholec, int k0, int q0, int q1) {
+    auto load_part = [&](auto stc, auto wholec, int k0, int rows, int q0, int q1) {
         constexpr int st = decltype(stc)::value % PF;
         constexpr bool whole = decltype(wholec)::value;
 #pragma unroll
         for (int q = q0; q < q1; ++q) {
-            ra[st][q] = get_a(q, k0, whole || k0 + ak0 + (akf ? 0 : q * QM) < kEnd);
+            ra[st][q] = get_a(q, rows, whole || k0 + ak0 + (akf ? 0 : q * QM) < kEnd);
             rb[st][q] = get_b(q, whole || k0 + bk0 + (bkf ? 0 : q * QM) < kEnd);
         }
     };
+    int rows = gathered(kb);            // of the K-tile to be asked for next
     auto advance = [&]() {
         Ab += da;
         Bb += db;
@@ -366,8 +387,11 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
                 constexpr int q0 = s * (NQ / MS), q1 = q0 + NQ / MS;
                 if (more) write_part(nextc, q0, q1);
                 if (ask) {
-                    load_part(nextc, std::bool_constant<!CHECK>{}, kl, q0, q1);
-                    if (s == MS - 1) advance();
+                    load_part(nextc, std::bool_constant<!CHECK>{}, kl, rows, q0, q1);
+                    if (s == MS - 1) {
+                        advance();
+                        rows = gathered(kl + BK);
+                    }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -393,15 +417,17 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
     if (tiles > 0) {
         constexpr auto b0 = std::integral_constant<int, 0>{};
         constexpr auto b1 = std::integral_constant<int, 1>{};
-        load_part(b0, std::false_type{}, kb, 0, NQ);
+        const int rows1 = gathered(kb + BK), rows2 = gathered(kb + PF * BK);
+        load_part(b0, std::false_type{}, kb, rows, 0, NQ);
         advance();
+        rows = gathered(kb + (PF + 1) * BK);
         if (PF == 2 && tiles > 1) {
-            load_part(b1, std::false_type{}, kb + BK, 0, NQ);
+            load_part(b1, std::false_type{}, kb + BK, rows1, 0, NQ);
             advance();
         }
         write_part(b0, 0, NQ);
         if (tiles > PF) {
-            load_part(std::integral_constant<int, PF>{}, std::false_type{}, kb + PF * BK, 0, NQ);
+            load_part(std::integral_constant<int, PF>{}, std::false_type{}, kb + PF * BK, rows2, 0, NQ);
             advance();
         }
         __syncthreads();
@@ -500,14 +526,14 @@ template <class T> int tile_layout(const ProductDesc& p, int mode, int tw)
                        (bm - 1) * p.sb_n + (BK - 1) * p.sb_k <= lim;
     const bool ak = p.sa_k == 1, bk = p.sb_k == 1;
     if (!off32 || (mode == PRODUCT_ROWS && !ak) || (mode == PRODUCT_SUM && (bk || (ak && !p.gather)))) return LAY_ANY;
-    return LAY_FAST | (ak && mode != PRODUCT_SUM ? LAY_A_K : 0) | (bk ? LAY_B_K : 0);
+    if (mode == PRODUCT_SUM) return LAY_FAST | (p.gather ? LAY_GATHER : 0);
+    return LAY_FAST | (ak ? LAY_A_K : 0) | (bk ? LAY_B_K : 0);
 }
 
 inline TileGrid tile_grid(const ProductDesc& p, int mode, int bm)
 {
     TileGrid g = {(unsigned)((p.m + bm - 1) / bm), (unsigned)((p.n + bm - 1) / bm), p.part ? (unsigned)p.nz : 1u};
-    // runs of rows: at most m / bm full tiles and one partial tile per run
-    if (mode == PRODUCT_ROWS) g.x = (unsigned)(p.m / bm + p.groups + (p.fill_rest ? 1 : 0));
+    if (mode == PRODUCT_ROWS) g.x = run_tiles(p, bm);
     if (mode == PRODUCT_SUM) g.z = (unsigned)p.groups;
     return g;
 }
@@ -530,7 +556,8 @@ int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
             if (lay == (AK | BK)) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK | BK>);
             else go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK>);
         } else {
-            go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST>);
+            if (p.gather) go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST | LAY_GATHER>);
+            else go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST>);
         }
     };
     if (lay == LAY_ANY) {                       // tiles of 64 only
@@ -554,7 +581,7 @@ bool product_pairs(const ProductDesc& p, int mode, int tw, const ProductDesc& q,
     const TileGrid g = tile_grid(p, mode, 32 * tw), h = tile_grid(q, qmode, 32 * tw);
     const double all = (double)g.x * g.y * g.z + (double)h.x * h.y * h.z;
     return tw == qtw && all < (1 << 23) && (mode == PRODUCT_DENSE ? qmode == PRODUCT_DENSE : mode == PRODUCT_ROWS && qmode == PRODUCT_SUM) &&
-           tile_layout<T>(p, mode, tw) == ABK && tile_layout<T>(q, qmode, tw) == LAY_FAST;
+           tile_layout<T>(p, mode, tw) == ABK && (tile_layout<T>(q, qmode, tw) & ~LAY_GATHER) == LAY_FAST;
 }
 
 template <class T>
@@ -564,14 +591,15 @@ int launch_product_pair(const ProductDesc& p, int mode, const ProductDesc& q, in
     const int qmode = mode == PRODUCT_DENSE ? PRODUCT_DENSE : PRODUCT_SUM;
     const ProductPair d = {p, q, tile_grid(p, mode, 32 * tw), tile_grid(q, qmode, 32 * tw)};
     const dim3 grid(d.gp.all() + d.gq.all());
-    if (mode == PRODUCT_DENSE && tw == 2)
-        hipLaunchKernelGGL((product_pair_kernel<T, 2, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>), grid, dim3(256), 0, st, d);
-    else if (mode == PRODUCT_DENSE)
-        hipLaunchKernelGGL((product_pair_kernel<T, 4, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>), grid, dim3(256), 0, st, d);
-    else if (tw == 2)
-        hipLaunchKernelGGL((product_pair_kernel<T, 2, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST>), grid, dim3(256), 0, st, d);
-    else
-        hipLaunchKernelGGL((product_pair_kernel<T, 4, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST>), grid, dim3(256), 0, st, d);
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, d); };
+    auto pick = [&](auto twc) {
+        constexpr int TW = decltype(twc)::value;
+        if (mode == PRODUCT_DENSE) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>);
+        else if (q.gather) go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST | LAY_GATHER>);
+        else go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST>);
+    };
+    if (tw == 2) pick(std::integral_constant<int, 2>{});
+    else pick(std::integral_constant<int, 4>{});
     LOCUS_HIP_CHECK(hipGetLastError());
     return 0;
 }

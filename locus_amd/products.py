@@ -29,6 +29,7 @@ from . import _lib
 ACTS = {"identity": 0, "logistic": 1, "probit": 2, "softplus": 3, "gelu": 4, "silu": 5}
 _DTYPES = {torch.float64: 0, torch.float32: 1}
 _DENSE, _ROWS = 0, 1
+_EWORKSPACE = -5                                 # LOCUS_HIP_EWORKSPACE
 _ARGS = struct.Struct("=3q6i2d26q")              # struct locus_hip_product_args
 _GRAD_ARGS = struct.Struct("=3q6id24q")          # struct locus_hip_product_grad_args
 
@@ -38,21 +39,28 @@ def _fail(msg):
 
 
 def _check(name, t, like, shape):
+    """`t` is a tensor of this shape beside `like` (its type, its device)."""
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is like.dtype and t.device == like.device:
+        return
     if not isinstance(t, torch.Tensor):
         _fail(f"{name} must be a tensor")
     if t.dtype != like.dtype or t.device != like.device:
         _fail(f"{name} must be a {like.dtype} tensor on {like.device}, not {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape:
-        _fail(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    _fail(f"{name} must have shape {shape}, not {tuple(t.shape)}")
 
 
-def _operand(name, t, dims):
-    if not isinstance(t, torch.Tensor) or t.dim() != dims:
-        _fail(f"{name} must be a {dims}-dimensional tensor")
-    if t.dtype not in _DTYPES:
-        _fail(f"{name}: float64 or float32, not {t.dtype}")
-    if t.device.type != "cuda":
-        _fail(f"{name} must be on the GPU (no CPU fallback)")
+def _operands(A, B, dims):
+    """Types and places of the two factors, B with `dims` dimensions; returns the type's number."""
+    for name, t, d in (("A", A, 2), ("B", B, dims)):
+        if not isinstance(t, torch.Tensor) or t.dim() != d:
+            _fail(f"{name} must be a {d}-dimensional tensor")
+    code = _DTYPES.get(A.dtype)
+    if code is None:
+        _fail(f"A: float64 or float32, not {A.dtype}")
+    if not A.is_cuda:
+        _fail("A must be on the GPU (no CPU fallback)")
+    _check("B", B, A, (*B.shape[:-2], A.shape[1], B.shape[-1]))
+    return code
 
 
 def _act(act):
@@ -62,49 +70,25 @@ def _act(act):
         _fail(f"act must be one of {', '.join(ACTS)}, not {act!r}")
 
 
-def _span(t):
-    """First and last byte of a tensor's elements."""
-    lo = t.data_ptr()
-    return lo, lo + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-
-
-def _apart(name, t, others):
-    """An output holds every element once and shares no memory with what the call reads."""
-    if t.numel() == 0:
-        return
-    reach = 1                                    # sizes by growing stride must not fold onto each other
-    for s, n in sorted(zip(t.stride(), t.shape)):
-        if n > 1:
-            if s < reach:
-                _fail(f"{name} has elements that share memory")
-            reach = s * (n - 1) + reach
-    lo, hi = _span(t)
-    for what, o in others:
-        if o is not None and o.numel() and o.element_size():
-            a, b = _span(o)
-            if a < hi and lo < b:
-                _fail(f"{name} shares memory with {what}")
-
-
 def _bias_strides(bias, like, m, n):
     """(stride over rows, stride over columns) of a bias per column (n,) / (1, n), per row (m, 1), one
     for all (1, 1) or a whole matrix (m, n)."""
     if not isinstance(bias, torch.Tensor):
         _fail("bias must be a tensor")
-    if bias.dtype != like.dtype or bias.device != like.device:
+    if bias.dtype is not like.dtype or bias.device != like.device:
         _fail(f"bias must be a {like.dtype} tensor on {like.device}")
-    shape = tuple(bias.shape)
+    shape = bias.shape
     if len(shape) == 1:
         if shape[0] != n:
             _fail(f"bias must have {n} entries, not {shape[0]}")
         return 0, bias.stride(0)
     if len(shape) != 2 or shape[0] not in (1, m) or shape[1] not in (1, n):
-        _fail(f"bias must have shape ({n},), ({m}, 1) or ({m}, {n}), not {shape}")
+        _fail(f"bias must have shape ({n},), ({m}, 1) or ({m}, {n}), not {tuple(shape)}")
     return (bias.stride(0) if shape[0] > 1 else 0), (bias.stride(1) if shape[1] > 1 else 0)
 
 
 def _index(name, t, like, size):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.device != like.device or t.dim() != 1:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int64 or t.device != like.device or t.dim() != 1:
         _fail(f"{name} must be a one-dimensional int64 tensor on {like.device}")
     if size is not None and t.shape[0] != size:
         _fail(f"{name} must have {size} entries, not {t.shape[0]}")
@@ -112,63 +96,58 @@ def _index(name, t, like, size):
         _fail(f"{name} must be contiguous")
 
 
-def _run(pack, need_fn, run_fn, fields, like):
-    """One call of the library: `fields` of the argument struct up to the workspace."""
-    need = need_fn(pack(*fields, 0, 0))
-    if need < 0:
-        _lib.check(int(need))
-    dev, ws = like.device, None
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    args = pack(*fields, ws.data_ptr() if need else 0, need)
-    if dev.index == torch.cuda.current_device():
-        _lib.check(run_fn(args, torch.cuda.current_stream(dev).cuda_stream))
-    else:
+def _run(pack, run_fn, need_fn, fields, dev):
+    """One call of the library on the current stream of `dev`: `fields` of the argument struct up to the
+    workspace, which is made when the library asks for one."""
+    if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            _lib.check(run_fn(args, torch.cuda.current_stream(dev).cuda_stream))
+            return _run(pack, run_fn, need_fn, fields, dev)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    rc = run_fn(pack(*fields, 0, 0), stream)
+    if rc == _EWORKSPACE:
+        need = need_fn(pack(*fields, 0, 0))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = run_fn(pack(*fields, ws.data_ptr(), need), stream)
+    if rc:
+        _lib.check(rc)
 
 
-def _forward(fields, like):
+def _forward(fields, dev):
     lib = _lib.lib()
-    _run(_ARGS.pack, lib.locus_hip_product_workspace_bytes, lib.locus_hip_product_dev, fields, like)
+    _run(_ARGS.pack, lib.locus_hip_product_dev, lib.locus_hip_product_workspace_bytes, fields, dev)
 
 
-def _strides(t):
-    return t.stride() if t is not None else (0, 0)
+def _at(t):
+    """Pointer and strides of a matrix that may be missing."""
+    return (0, 0, 0) if t is None else (t.data_ptr(), *t.stride())
 
 
 def _ptr(t):
-    return t.data_ptr() if t is not None else 0
+    return 0 if t is None else t.data_ptr()
 
 
 def _grouped_sizes(A, B, offsets, gather):
-    _operand("A", A, 2)
-    _operand("B", B, 3)
+    code = _operands(A, B, 3)
     m, k = A.shape
     groups, _, n = B.shape
-    _check("B", B, A, (groups, k, n))
     if groups < 1:
         _fail("B must hold at least one group")
     _index("offsets", offsets, A, groups + 1)
     if gather is not None:
         _index("gather", gather, A, None)
         m = gather.shape[0]
-    return m, n, k, groups
+    return code, m, n, k, groups
 
 
-def _outputs(A, m, n, out, pre, residual, reads):
-    """Checks or makes C; returns it."""
+def _outputs(A, m, n, out, pre, residual):
+    """Checks or makes C; returns it.  (That outputs share no memory with what is read is the library's check.)"""
     if residual is not None:
         _check("residual", residual, A, (m, n))
-    if out is None:
-        out = torch.empty((m, n), dtype=A.dtype, device=A.device)
-    else:
-        _check("out", out, A, (m, n))
-        same = residual is not None and out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()
-        _apart("out", out, reads + ([] if same else [("residual", residual)]))
     if pre is not None:
         _check("pre", pre, A, (m, n))
-        _apart("pre", pre, reads + [("residual", residual), ("out", out)])
+    if out is None:
+        return A.new_empty((m, n))
+    _check("out", out, A, (m, n))
     return out
 
 
@@ -180,18 +159,15 @@ def dense_product(A, B, bias=None, act="identity", residual=None, alpha=1.0, bet
     be the residual itself (the same memory and strides), and shares no memory with anything else.
     pre (m x n), when given, receives Z = alpha A B + bias, which dense_product_grad asks for.  cfg: the
     kernel's geometry (see include/locus_hip.h), (0, 0) = automatic."""
-    _operand("A", A, 2)
-    _operand("B", B, 2)
+    dtype = _operands(A, B, 2)
     m, k = A.shape
     n = B.shape[1]
-    _check("B", B, A, (k, n))
     code = _act(act)
     sbias = _bias_strides(bias, A, m, n) if bias is not None else (0, 0)
-    out = _outputs(A, m, n, out, pre, residual, [("A", A), ("B", B), ("bias", bias)])
+    out = _outputs(A, m, n, out, pre, residual)
     if m and n:
-        _forward((m, n, k, _DTYPES[A.dtype], code, _DENSE, 0, *cfg, alpha, beta, A.data_ptr(), *A.stride(),
-                  B.data_ptr(), *B.stride(), _ptr(bias), *sbias, _ptr(residual), *_strides(residual),
-                  out.data_ptr(), *out.stride(), _ptr(pre), *_strides(pre), 0, 0, 0, 0, 0, 0), A)
+        _forward((m, n, k, dtype, code, _DENSE, 0, *cfg, alpha, beta, A.data_ptr(), *A.stride(), B.data_ptr(),
+                  *B.stride(), _ptr(bias), *sbias, *_at(residual), *_at(out), *_at(pre), 0, 0, 0, 0, 0, 0), A.device)
     return out
 
 
@@ -203,45 +179,47 @@ def grouped_product(A, B, offsets, bias=None, act="identity", residual=None, alp
     B (groups x k x n), bias (groups x n).  C has as many rows as `gather`, else as A; they are in the order of
     the runs (gathered rows are not moved back).  Runs may be empty.  Rows of no run are 0 in an `out` that
     is made here, and are left as they were in one that is given (and in its `pre`)."""
-    m, n, k, groups = _grouped_sizes(A, B, offsets, gather)
+    dtype, m, n, k, groups = _grouped_sizes(A, B, offsets, gather)
     code = _act(act)
     if bias is not None:
         _check("bias", bias, A, (groups, n))
     fill = out is None
-    out = _outputs(A, m, n, out, pre, residual, [("A", A), ("B", B), ("bias", bias), ("offsets", offsets),
-                                                 ("gather", gather)])
+    out = _outputs(A, m, n, out, pre, residual)
     if m and n:
         sb = B.stride()
         sbias = bias.stride() if bias is not None else (0, 0)
-        _forward((m, n, k, _DTYPES[A.dtype], code, _ROWS, int(fill), *cfg, alpha, beta, A.data_ptr(), *A.stride(),
-                  B.data_ptr(), sb[1], sb[2], _ptr(bias), 0, sbias[1], _ptr(residual), *_strides(residual),
-                  out.data_ptr(), *out.stride(), _ptr(pre), *_strides(pre), groups, offsets.data_ptr(), sb[0],
-                  sbias[0], _ptr(gather), A.shape[0]), A)
+        _forward((m, n, k, dtype, code, _ROWS, fill, *cfg, alpha, beta, A.data_ptr(), *A.stride(), B.data_ptr(), sb[1],
+                  sb[2], _ptr(bias), 0, sbias[1], *_at(residual), *_at(out), *_at(pre), groups, offsets.data_ptr(),
+                  sb[0], sbias[0], _ptr(gather), A.shape[0]), A.device)
     return out
 
 
-def _gradient(dC, A, B, act, pre, alpha, need_A, need_B, bias_grad, m, n, k, groups, offsets, gather, cfg):
+def _gradient(dC, A, B, dtype, act, pre, alpha, need_A, need_B, bias_grad, m, n, k, groups, offsets, gather, cfg):
     code = _act(act)
     _check("dC", dC, A, (m, n))
     if code:
         if pre is None:
             _fail(f"the gradient of {act!r} needs pre, the Z kept by the forward call")
         _check("pre", pre, A, (m, n))
-    new = lambda *shape: torch.empty(shape, dtype=A.dtype, device=A.device)  # noqa: E731
     runs = (groups,) if groups else ()
-    dA = new(m, k) if need_A else None
-    dB = new(*runs, k, n) if need_B else None
-    db = {"column": lambda: new(*runs, n), "row": lambda: new(m, 1), "matrix": lambda: new(m, n) if code else dC.clone(),
-          None: lambda: None}[bias_grad]()
+    dA = A.new_empty((m, k)) if need_A else None
+    dB = A.new_empty((*runs, k, n)) if need_B else None
+    G = cols = rows = None                      # of the bias: whole, summed over rows, summed over columns
+    if bias_grad == "column":
+        cols = A.new_empty((*runs, n))
+    elif bias_grad == "row":
+        rows = A.new_empty((m, 1))
+    elif bias_grad == "matrix" and code:
+        G = A.new_empty((m, n))
     sb = B.stride()
     lib = _lib.lib()
-    _run(_GRAD_ARGS.pack, lib.locus_hip_product_grad_workspace_bytes, lib.locus_hip_product_grad_dev,
-         (m, n, k, _DTYPES[A.dtype], code, _ROWS if groups else _DENSE, 0, *cfg, alpha, dC.data_ptr(), *dC.stride(),
-          _ptr(pre) if code else 0, *_strides(pre), A.data_ptr(), *A.stride(), B.data_ptr(), sb[-2], sb[-1],
-          _ptr(db) if bias_grad == "matrix" and code else 0, _ptr(dA), _ptr(dB), _ptr(db) if bias_grad == "column" else 0,
-          _ptr(db) if bias_grad == "row" else 0, groups, _ptr(offsets), sb[0] if groups else 0, _ptr(gather),
-          A.shape[0]), A)
-    return dA, dB, db
+    _run(_GRAD_ARGS.pack, lib.locus_hip_product_grad_dev, lib.locus_hip_product_grad_workspace_bytes,
+         (m, n, k, dtype, code, _ROWS if groups else _DENSE, 0, *cfg, alpha, *_at(dC), *_at(pre if code else None),
+          *_at(A), B.data_ptr(), sb[-2], sb[-1], _ptr(G), _ptr(dA), _ptr(dB), _ptr(cols), _ptr(rows), groups,
+          _ptr(offsets), sb[0] if groups else 0, _ptr(gather), A.shape[0]), A.device)
+    if bias_grad == "matrix":
+        return dA, dB, G if code else dC.clone()
+    return dA, dB, cols if cols is not None else rows
 
 
 def dense_product_grad(dC, A, B, act="identity", pre=None, alpha=1.0, need_A=True, need_B=True, bias_grad=None,
@@ -251,14 +229,12 @@ def dense_product_grad(dC, A, B, act="identity", pre=None, alpha=1.0, need_A=Tru
     dbias = G summed to the shape of the bias: bias_grad = "column" (n,), "row" (m, 1), "matrix" (m, n) or
     None.  pre is what the forward call stored; the identity needs none.  The residual's gradient is
     beta dC."""
-    _operand("A", A, 2)
-    _operand("B", B, 2)
+    dtype = _operands(A, B, 2)
     m, k = A.shape
     n = B.shape[1]
-    _check("B", B, A, (k, n))
     if bias_grad not in (None, "column", "row", "matrix"):
         _fail(f"bias_grad must be None, 'column', 'row' or 'matrix', not {bias_grad!r}")
-    return _gradient(dC, A, B, act, pre, alpha, need_A, need_B, bias_grad, m, n, k, 0, None, None, cfg)
+    return _gradient(dC, A, B, dtype, act, pre, alpha, need_A, need_B, bias_grad, m, n, k, 0, None, None, cfg)
 
 
 def grouped_product_grad(dC, A, B, offsets, act="identity", pre=None, alpha=1.0, gather=None, need_A=True,
@@ -268,6 +244,6 @@ def grouped_product_grad(dC, A, B, offsets, act="identity", pre=None, alpha=1.0,
         dB[g] = alpha sum_{r in g} A[src(r)]' G[r],  dbias[g] = sum_{r in g} G[r].
     dA has a row for each row of dC: with `gather` it is in the order of the runs, and the gradient of A's
     row i is the sum of the dA[r] with gather[r] = i.  Rows of no run: 0 in dA.  Empty runs: 0 in dB."""
-    m, n, k, groups = _grouped_sizes(A, B, offsets, gather)
-    return _gradient(dC, A, B, act, pre, alpha, need_A, need_B, "column" if need_bias else None, m, n, k, groups, offsets,
-                     gather, cfg)
+    dtype, m, n, k, groups = _grouped_sizes(A, B, offsets, gather)
+    return _gradient(dC, A, B, dtype, act, pre, alpha, need_A, need_B, "column" if need_bias else None, m, n, k, groups,
+                     offsets, gather, cfg)
