@@ -146,16 +146,12 @@ Plan plan_product(const Want& w)
     Plan pl;
     const ProductDesc& p = w.p;
     const long M = p.m, N = p.n, K = p.k, s = w.f64 ? 8 : 4, bk = w.f64 ? 16 : 32;
-    const bool runs = w.mode == PRODUCT_ROWS;
+    const bool runs = w.mode == PRODUCT_ROWS, sums = w.mode == PRODUCT_SUM;
     const double avg = runs ? (double)M / p.groups : (double)M;
+    const long copies = sums ? p.groups : 1, len = sums ? (K + copies - 1) / copies : K;   // a sum's length
     pl.kchunk = K;
-    if (w.mode == PRODUCT_SUM) {
-        const long t128 = ((M + 127) / 128) * ((N + 127) / 128) * p.groups;
-        pl.tw = w.cfg[0] >= 64 ? w.cfg[0] / 32 : (t128 >= 8 * w.cus ? 4 : 2);
-        return pl;
-    }
     const long side = runs ? (long)avg : std::min(M, N);
-    pl.rows = w.cfg[0] ? w.cfg[0] == 16 : side <= w.few && (runs || std::max(M, N) * K >= w.large);
+    if (!sums) pl.rows = w.cfg[0] ? w.cfg[0] == 16 : side <= w.few && (runs || std::max(M, N) * K >= w.large);
     if (pl.rows) {
         pl.swap = !runs && N < M;
         const long m = pl.swap ? N : M, n = pl.swap ? M : N, kb = w.f64 ? 8 : 16;
@@ -177,14 +173,14 @@ Plan plan_product(const Want& w)
     const double heavy = p.epi.act == LOCUS_HIP_ACT_IDENTITY ? 0.0 : (w.f64 ? (cdf ? 2200.0 : 1000.0) : 400.0);
     double best = 1e300;
     for (int tw = 4; tw >= 2; tw -= 2) {
-        if (w.cfg[0] && w.cfg[0] != 32 * tw) continue;
+        if (w.cfg[0] >= 64 && w.cfg[0] != 32 * tw) continue;
         const long bm = 32 * tw;
         const long mt = runs ? p.groups * ((long)(avg + bm - 1) / bm) : (M + bm - 1) / bm;
-        const long tiles = std::max<long>(mt, 1) * ((N + bm - 1) / bm);
+        const long tiles = std::max<long>(mt, 1) * ((N + bm - 1) / bm) * copies;
         for (long nz = w.cfg[1] ? w.cfg[1] : 1; nz <= (w.cfg[1] ? w.cfg[1] : 32); ++nz) {
-            const long chunk = ((K + nz - 1) / nz + bk - 1) / bk * bk;
+            const long chunk = ((len + nz - 1) / nz + bk - 1) / bk * bk;
             if (!w.cfg[1] && nz > 1 && chunk < 4 * bk) break;
-            const long used = K > 0 ? (K + chunk - 1) / chunk : 1;
+            const long used = sums ? nz : (K > 0 ? (K + chunk - 1) / chunk : 1);
             const long wgs = tiles * used, load = (wgs + w.cus - 1) / w.cus, slots = tw == 4 ? 2 : 4;
             static const double share2[5] = {0, 0.67, 0.80, 0.86, 0.90}, share4[3] = {0, 0.86, 0.92};
             const double* share = tw == 4 ? share4 : share2;
@@ -195,7 +191,7 @@ Plan plan_product(const Want& w)
             // the element function: in the epilogue by a CU's workgroups, after a split by all CUs
             const double f = 1e-6 * bm * bm * heavy;
             t += used == 1 ? f * std::max<double>(1.0, (double)wgs / w.cus / 2) : f * tiles / w.cus / 2;
-            if (used > 1) t += 4.0 + 2.0 * used * M * N * s / 4.5e6;
+            if (used > 1) t += 4.0 + 2.0 * used * M * N * copies * s / 4.5e6;
             if (t < best) {
                 best = t;
                 pl.tw = tw;
@@ -209,7 +205,8 @@ Plan plan_product(const Want& w)
 
 long plan_bytes(const Want& w, const Plan& pl)
 {
-    return pl.nz > 1 ? (long)pl.nz * w.p.m * w.p.n * (w.f64 ? 8 : 4) : 0;
+    const long copies = w.mode == PRODUCT_SUM ? w.p.groups : 1;
+    return pl.nz > 1 ? (long)pl.nz * w.p.m * w.p.n * copies * (w.f64 ? 8 : 4) : 0;
 }
 
 // The descriptor as the kernels take it: roles swapped, split sum in `part`.
@@ -228,11 +225,11 @@ ProductDesc planned(const Want& w, const Plan& pl, void* part)
         std::swap(e.sr_m, e.sr_n);
         std::swap(e.sp_m, e.sp_n);
     }
-    p.nz = pl.nz;
+    p.nz = std::max(1, pl.nz);
     p.kchunk = (int)pl.kchunk;
     if (pl.nz > 1) {
         p.part = part;
-        p.part_z = (long)p.m * p.n;
+        p.part_z = (long)p.m * p.n * (w.mode == PRODUCT_SUM ? p.groups : 1);
         const bool mfast = w.mode == PRODUCT_DENSE && e.sc_n != 1 && e.sc_m == 1 && !pl.rows;
         p.part_m = mfast ? 1 : p.n;
         p.part_n = mfast ? p.m : 1;
@@ -240,9 +237,13 @@ ProductDesc planned(const Want& w, const Plan& pl, void* part)
     return p;
 }
 
-template <class T> int join_product(const ProductDesc& p, int mode, hipStream_t st)
+template <class T> int join_product(ProductDesc p, int mode, hipStream_t st)
 {
     if (p.nz <= 1) return 0;
+    if (mode == PRODUCT_SUM) {                 // the runs' C lie one behind the other, as their partials do
+        p.m *= p.groups;
+        mode = PRODUCT_DENSE;
+    }
     const dim3 grid(grid_of(((long)p.m * p.n + 255) / 256));
     if (mode == PRODUCT_DENSE) hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_DENSE>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((product_join_kernel<T, PRODUCT_ROWS>), grid, dim3(256), 0, st, p);
@@ -448,6 +449,7 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     q.epi.C = a.dB; q.epi.sc_m = a.n; q.epi.sc_n = 1;
     q.sc_g = a.k * a.n;
     if (runs) { q.gather = a.gather; q.a_rows = a.a_rows; }
+    if (a.k * std::max<long>(1, a.groups) >= (1l << 31)) r.db.cfg[1] = 1;       // dB's rows are counted in 32 bits
     if (a.dA) r.pa = plan_product(r.da);
     if (a.dB) r.pb = plan_product(r.db);
     if (a.dA && a.dB && !r.pa.rows && !r.pb.rows && r.pa.tw != r.pb.tw) {   // one launch wants one tile

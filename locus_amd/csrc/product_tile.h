@@ -73,7 +73,7 @@ __device__ __forceinline__ void store_block(const ProductDesc& p, const T* lds, 
         return static_cast<T*>(const_cast<void*>(base)) + off + gi * sm + gj * sn;
     };
     const long c_m = raw ? p.part_m : e.sc_m, c_n = raw ? p.part_n : e.sc_n;
-    T* c = walk(raw ? p.part : e.C, raw ? bz * p.part_z : c0, c_m, c_n);
+    T* c = walk(raw ? p.part : e.C, raw ? bz * p.part_z + c0 : c0, c_m, c_n);
     const long c_f = mfast ? c_m : c_n, c_s = sp * (mfast ? c_n : c_m);
     const T* res = walk(e.res, 0, e.sr_m, e.sr_n);
     const long r_f = mfast ? e.sr_m : e.sr_n, r_s = sp * (mfast ? e.sr_n : e.sr_m);
@@ -226,15 +226,19 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
         B += r.g * p.sb_g;
         bias0 = r.g * p.sbias_g;
     } else {
-        const Run r = run_rows(p.offsets, p.k, bz);
+        // a run's rows in nz parts of whole K-tiles
+        const unsigned g = bz / (unsigned)p.nz;
+        bz -= g * p.nz;
+        const Run r = run_rows(p.offsets, p.k, g);
+        const int len = r.hi - r.lo, chunk = (len + p.nz * BK - 1) / (p.nz * BK) * BK;
         m0 = (long)bx * BM;
         mEnd = p.m;
-        kb = r.lo;
-        kEnd = r.hi;
-        c0 = r.g * p.sc_g;
-        if (kb >= kEnd) {               // an empty run: 0
+        kb = r.lo + (int)bz * chunk;
+        kEnd = kb + chunk < r.hi ? kb + chunk : r.hi;
+        c0 = g * p.sc_g;
+        if (kb >= kEnd) {               // no rows: 0
             const int w = nEnd - n0 < BN ? nEnd - n0 : BN;
-            T* C = static_cast<T*>(p.epi.C) + c0 + m0 * p.epi.sc_m + n0;
+            T* C = static_cast<T*>(p.part ? p.part : p.epi.C) + (p.part ? bz * p.part_z : 0) + c0 + m0 * p.epi.sc_m + n0;
             const int h = (int)(mEnd - m0 < BM ? mEnd - m0 : BM);
             if (w == p.epi.sc_m) {      // whole rows: one piece of memory
                 for (int e = tid; e < h * w; e += 256) C[e] = T(0);
@@ -534,7 +538,7 @@ inline TileGrid tile_grid(const ProductDesc& p, int mode, int bm)
 {
     TileGrid g = {(unsigned)((p.m + bm - 1) / bm), (unsigned)((p.n + bm - 1) / bm), p.part ? (unsigned)p.nz : 1u};
     if (mode == PRODUCT_ROWS) g.x = run_tiles(p, bm);
-    if (mode == PRODUCT_SUM) g.z = (unsigned)p.groups;
+    if (mode == PRODUCT_SUM) g.z = (unsigned)p.groups * (unsigned)p.nz;
     return g;
 }
 
