@@ -305,11 +305,11 @@ int locus_hip_gemm_dev(int64_t m, int64_t n, int64_t k, double alpha, const doub
 #define LOCUS_HIP_PRODUCT_DENSE 0
 #define LOCUS_HIP_PRODUCT_ROWS 1
 typedef struct locus_hip_product_args {
-    int64_t m, n, k;            /* m, k < 2^30, n <= 4194240                                    */
+    int64_t m, n, k;            /* m, k < 2^29, n <= 4194240                                    */
     int32_t dtype, act, mode, fill_rest;
     int32_t cfg[2];             /* kernel geometry, 0 = automatic: cfg[0] = 16 (kernel for few rows),
                                    64, 128 (tiles of so many rows and columns); cfg[1] = slices of k
-                                   (1..256)                                                     */
+                                   (1..256; gradients: as many as runs x slices <= 65535 leave) */
     double alpha, beta;
     const void* A; int64_t sa_m, sa_k;
     const void* B; int64_t sb_k, sb_n;
@@ -332,7 +332,8 @@ int64_t locus_hip_product_workspace_bytes(const locus_hip_product_args* args);
  *   G = dC act'(pre),  dA = alpha G B' (m x k),  dB = alpha A' G (k x n; ROWS: [groups][k][n], 0 for an
  *   empty run),  col_sums[n] (ROWS: [groups][n]) = G summed over rows, the gradient of a bias per
  *   column;  row_sums[m] (DENSE) = G summed over columns, of a bias per row;  G itself, of a whole matrix.
- * Outputs are row-major, each NULL where it is not wanted; for the identity G is dC (pass NULL).  The
+ * Outputs are row-major, each NULL where it is not wanted, and share no memory with each other or with
+ * what is read (else LOCUS_HIP_EINVAL); for the identity G is dC (pass NULL).  The
  * gradient of res is beta dC.  ROWS: rows of no run are 0 in dA and not written in G; with gather dA
  * stays in the order of the runs (the gradient of A's row i is the sum of the dA[r] with gather[r] = i). */
 typedef struct locus_hip_product_grad_args {

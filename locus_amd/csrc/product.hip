@@ -177,7 +177,9 @@ Plan plan_product(const Want& w)
         const long bm = 32 * tw;
         const long mt = runs ? p.groups * ((long)(avg + bm - 1) / bm) : (M + bm - 1) / bm;
         const long tiles = std::max<long>(mt, 1) * ((N + bm - 1) / bm) * copies;
-        for (long nz = w.cfg[1] ? w.cfg[1] : 1; nz <= (w.cfg[1] ? w.cfg[1] : 32); ++nz) {
+        const long most = 65535 / copies;                              // runs x parts: a grid's third axis
+        const long asked = std::min<long>(w.cfg[1], most);
+        for (long nz = asked ? asked : 1; nz <= (asked ? asked : std::min<long>(32, most)); ++nz) {
             const long chunk = ((len + nz - 1) / nz + bk - 1) / bk * bk;
             if (!w.cfg[1] && nz > 1 && chunk < 4 * bk) break;
             const long used = sums ? nz : (K > 0 ? (K + chunk - 1) / chunk : 1);
@@ -266,12 +268,12 @@ int check_common(const char* what, int64_t m, int64_t n, int64_t k, int dtype, i
     LOCUS_REQUIRE(dtype == LOCUS_HIP_F64 || dtype == LOCUS_HIP_F32, w + ": dtype");
     LOCUS_REQUIRE(act >= LOCUS_HIP_ACT_IDENTITY && act <= LOCUS_HIP_ACT_SILU, w + ": act");
     LOCUS_REQUIRE(mode == LOCUS_HIP_PRODUCT_DENSE || mode == LOCUS_HIP_PRODUCT_ROWS, w + ": mode");
-    LOCUS_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < (1ll << 30) && n <= 65535 * 64 && k < (1ll << 30),
-                  w + ": sizes (m, k < 2^30, n <= 4194240)");
+    LOCUS_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < (1ll << 29) && n <= 65535 * 64 && k < (1ll << 29),
+                  w + ": sizes (m, k < 2^29, n <= 4194240)");
     LOCUS_REQUIRE(cfg[0] == 0 || cfg[0] == 16 || cfg[0] == 64 || cfg[0] == 128, w + ": cfg[0] is 0, 16, 64 or 128");
     LOCUS_REQUIRE(cfg[1] >= 0 && cfg[1] <= 256, w + ": cfg[1] is 0..256");
-    LOCUS_REQUIRE(cfg[0] != 16 || mode != LOCUS_HIP_PRODUCT_DENSE || std::min(m, n) < (1ll << 20),
-                  w + ": the kernel for few rows takes fewer than 2^20 of them");
+    LOCUS_REQUIRE(cfg[0] != 16 || (mode == LOCUS_HIP_PRODUCT_DENSE ? std::min(m, n) <= 65535 * 16 : m < (1ll << 27)),
+                  w + ": too many rows for the kernel for few");
     if (mode == LOCUS_HIP_PRODUCT_ROWS) {
         LOCUS_REQUIRE(groups >= 1 && groups <= 65535, w + ": groups (1..65535)");
         LOCUS_REQUIRE(!gather || (a_rows >= 0 && a_rows < (1ll << 31)), w + ": a_rows");
@@ -294,18 +296,49 @@ int check_product(const locus_hip_product_args* a)
 // The bytes that a strided array spans.
 struct Span {
     const char *lo = nullptr, *hi = nullptr;
-    Span(const void* at, long size, std::initializer_list<std::pair<long, long>> dims)
+    const char* at = nullptr;
+    long size = 0, n[3] = {1, 1, 1}, s[3] = {0, 0, 0};
+    Span(const void* p, long bytes, std::initializer_list<std::pair<long, long>> dims)
     {
-        if (!at) return;
+        if (!p) return;
         long back = 0, ahead = 0;
-        for (auto [n, s] : dims) {
-            if (n == 0) return;
-            (s < 0 ? back : ahead) += (n - 1) * s;
+        int q = 0;
+        for (auto [len, step] : dims) {
+            if (len == 0) return;
+            n[q] = len;
+            s[q++] = step * bytes;
+            (step < 0 ? back : ahead) += (len - 1) * step;
         }
-        lo = static_cast<const char*>(at) + back * size;
-        hi = static_cast<const char*>(at) + (ahead + 1) * size;
+        at = static_cast<const char*>(p);
+        size = bytes;
+        lo = at + back * bytes;
+        hi = at + (ahead + 1) * bytes;
     }
-    bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+    // [from, to): where the array's bytes lie within a period, counted from `at`; dimensions whose stride is a
+    // whole number of periods do not count
+    std::pair<long, long> within(long period) const
+    {
+        long from = 0, to = size;
+        for (int q = 0; q < 3; ++q)
+            if (s[q] % period) (s[q] < 0 ? from : to) += (n[q] - 1) * s[q];
+        return {from, to};
+    }
+    // Blocks of columns of one matrix lie within each other's span and share nothing: with the matrix's row
+    // as the period, one begins behind the other's end and ends before its next row.
+    bool meets(const Span& o) const
+    {
+        if (!(lo < o.hi && o.lo < hi)) return false;
+        for (const Span* x : {this, &o})
+            for (int q = 0; q < 3; ++q) {
+                const long period = x->s[q] < 0 ? -x->s[q] : x->s[q];
+                if (x->n[q] < 2 || period <= size) continue;
+                const auto [a0, a1] = within(period);
+                const auto [b0, b1] = o.within(period);
+                const long gap = (((long)(o.at - at) + b0 - a0) % period + period) % period;
+                if (gap >= a1 - a0 && gap + (b1 - b0) <= period) return false;
+            }
+        return true;
+    }
 };
 
 // Rows (or columns) that lie one behind the other: every element has memory of its own.
@@ -394,6 +427,34 @@ int check_grad(const locus_hip_product_grad_args* a)
     LOCUS_REQUIRE(!(a->row_sums && a->mode == LOCUS_HIP_PRODUCT_ROWS), "product_grad: row sums are for one pair of matrices");
     LOCUS_REQUIRE(!(a->G && a->act == LOCUS_HIP_ACT_IDENTITY), "product_grad: with act = identity, G is dC: pass NULL");
     return 0;
+}
+
+int check_grad_spans(const locus_hip_product_grad_args& a)
+{
+    const long s = a.dtype == LOCUS_HIP_F64 ? 8 : 4, groups = std::max<long>(1, a.groups);
+    const Span writes[] = {Span(a.G, s, {{a.m, a.n}, {a.n, 1}}), Span(a.dA, s, {{a.m, a.k}, {a.k, 1}}),
+                           Span(a.dB, s, {{groups * a.k, a.n}, {a.n, 1}}), Span(a.col_sums, s, {{groups, a.n}, {a.n, 1}}),
+                           Span(a.row_sums, s, {{a.m, 1}})};
+    const Span reads[] = {Span(a.dC, s, {{a.m, a.sd_m}, {a.n, a.sd_n}}),
+                          Span(a.act != LOCUS_HIP_ACT_IDENTITY ? a.pre : nullptr, s, {{a.m, a.sp_m}, {a.n, a.sp_n}}),
+                          Span(a.dB ? a.A : nullptr, s, {{a.gather ? a.a_rows : a.m, a.sa_m}, {a.k, a.sa_k}}),
+                          Span(a.dA ? a.B : nullptr, s, {{groups, a.sb_g}, {a.k, a.sb_k}, {a.n, a.sb_n}}),
+                          Span(a.offsets, 8, {{groups + 1, 1}}), Span(a.gather, 8, {{a.m, 1}})};
+    for (const Span& w : writes) {
+        for (const Span& r : reads) LOCUS_REQUIRE(!w.meets(r), "product_grad: an output shares memory with what is read");
+        for (const Span& o : writes) LOCUS_REQUIRE(&o == &w || !w.meets(o), "product_grad: two outputs share memory");
+    }
+    return 0;
+}
+
+// One pair of matrices has no runs, whatever those fields hold.
+locus_hip_product_grad_args own_fields(locus_hip_product_grad_args a)
+{
+    if (a.mode == LOCUS_HIP_PRODUCT_DENSE) {
+        a.groups = a.sb_g = a.a_rows = 0;
+        a.offsets = a.gather = nullptr;
+    }
+    return a;
 }
 
 // What a gradient launches: workspace [G | column sums | partials of dA | partials of dB].
@@ -541,14 +602,14 @@ int locus_hip_product_dev(const locus_hip_product_args* args, void* stream)
 int64_t locus_hip_product_grad_workspace_bytes(const locus_hip_product_grad_args* args)
 {
     const int rc = check_grad(args);
-    return rc ? rc : plan_grad(*args).all();
+    return rc ? rc : plan_grad(own_fields(*args)).all();
 }
 
 int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* stream)
 {
     int rc = check_grad(args);
     if (rc) return rc;
-    const locus_hip_product_grad_args& a = *args;
+    const locus_hip_product_grad_args a = own_fields(*args);
     const bool act = a.act != LOCUS_HIP_ACT_IDENTITY;
     LOCUS_REQUIRE(a.m == 0 || a.n == 0 || (a.dC && (!act || a.pre)), "product_grad: null pointer");
     LOCUS_REQUIRE(!a.dA || a.B || a.k == 0 || a.n == 0 || a.m == 0, "product_grad: dA needs B");
@@ -556,6 +617,7 @@ int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* st
     LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || a.offsets, "product_grad: runs need offsets");
     LOCUS_REQUIRE(a.mode == LOCUS_HIP_PRODUCT_DENSE || !a.gather || a.a_rows > 0 || a.m == 0 || a.k == 0,
                   "product_grad: rows gathered from an empty matrix");
+    if ((rc = check_grad_spans(a))) return rc;
     Grad r = plan_grad(a);
     if (r.all() > (a.workspace ? a.workspace_bytes : 0)) return no_workspace("locus_hip_product_grad_workspace_bytes()");
     return a.dtype == LOCUS_HIP_F64 ? run_grad<double>(a, r, (hipStream_t)stream) : run_grad<float>(a, r, (hipStream_t)stream);

@@ -38,10 +38,16 @@ def _fail(msg):
     raise ValueError(msg)
 
 
+def _plain(name, t):
+    """Memory holds the values themselves (a conjugate's imaginary part, say, is kept with its sign pending)."""
+    if t.is_neg():
+        _fail(f"{name} is a negated view: pass {name}.resolve_neg()")
+
+
 def _check(name, t, like, shape):
     """`t` is a tensor of this shape beside `like` (its type, its device)."""
     if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is like.dtype and t.device == like.device:
-        return
+        return _plain(name, t)
     if not isinstance(t, torch.Tensor):
         _fail(f"{name} must be a tensor")
     if t.dtype != like.dtype or t.device != like.device:
@@ -54,6 +60,7 @@ def _operands(A, B, dims):
     for name, t, d in (("A", A, 2), ("B", B, dims)):
         if not isinstance(t, torch.Tensor) or t.dim() != d:
             _fail(f"{name} must be a {d}-dimensional tensor")
+    _plain("A", A)
     code = _DTYPES.get(A.dtype)
     if code is None:
         _fail(f"A: float64 or float32, not {A.dtype}")
@@ -77,6 +84,7 @@ def _bias_strides(bias, like, m, n):
         _fail("bias must be a tensor")
     if bias.dtype is not like.dtype or bias.device != like.device:
         _fail(f"bias must be a {like.dtype} tensor on {like.device}")
+    _plain("bias", bias)
     shape = bias.shape
     if len(shape) == 1:
         if shape[0] != n:

@@ -40,7 +40,9 @@ BAD = [dict(dtype=2), dict(act=6), dict(act=-1), dict(mode=2), dict(m=-1), dict(
        dict(res=(3 << 20) + 8, sr_m=3, sr_n=1), dict(res=3 << 20, sr_m=1, sr_n=4)]
 BAD_GRAD = [dict(dtype=-1), dict(act=7), dict(mode=3), dict(k=4194241), dict(cfg0=1), dict(act=1), dict(dC=0), dict(A=0),
             dict(B=0), dict(G=6 << 20), dict(mode=1, groups=1, offsets=7 << 20, row_sums=6 << 20), dict(mode=1, groups=1),
-            dict(mode=1, groups=2, offsets=7 << 20, gather=8 << 20, a_rows=0)]
+            dict(mode=1, groups=2, offsets=7 << 20, gather=8 << 20, a_rows=0),
+            dict(dA=(1 << 20) + 88), dict(dB=(2 << 20) - 16), dict(dB=(4 << 20) + 8), dict(col_sums=(3 << 20) + 8),
+            dict(row_sums=5 << 20)]
 
 
 @pytest.mark.parametrize("kw", BAD, ids=str)
@@ -74,6 +76,24 @@ def test_null_arguments_and_missing_workspace(monkeypatch):
     assert lib.locus_hip_product_grad_dev(grad(**g), None) == EWORKSPACE
 
 
+@pytest.mark.parametrize("at,ok", [(512, True), (504, False), (1000, True), (1008, False), (1016, False), (1024, False),
+                                   (1536, True), (2024, True), (-24, True), (-16, False), (-1024 + 512, True)])
+def test_blocks_of_one_matrix_share_no_memory(monkeypatch, at, ok):
+    """A: columns 0 .. 63 of rows of 128 (1024 bytes), C: 3 other columns `at` bytes from there, or not quite.  (The
+    missing workspace stops the calls that pass.)"""
+    monkeypatch.setenv("LOCUS_HIP_MFMA_CUS", "256")
+    lib = _lib.lib()
+    rc = lib.locus_hip_product_dev(args(m=4, n=3, k=64, sa_m=128, sc_m=128, C=(1 << 20) + at, cfg0=64, cfg1=4), None)
+    assert rc == (EWORKSPACE if ok else EINVAL)
+
+
+def test_a_dense_gradient_has_no_runs(monkeypatch):
+    monkeypatch.setenv("LOCUS_HIP_MFMA_CUS", "256")
+    need = _lib.lib().locus_hip_product_grad_workspace_bytes
+    big = dict(m=5000, n=70, k=30, act=1, pre=1 << 40, sp_m=70, sp_n=1, col_sums=1 << 41)
+    assert need(grad(**big)) == need(grad(**big, groups=900, offsets=1 << 42, gather=1 << 43, a_rows=9)) > 0
+
+
 def test_empty_products_do_nothing(monkeypatch):
     monkeypatch.setenv("LOCUS_HIP_MFMA_CUS", "256")
     lib = _lib.lib()
@@ -96,6 +116,8 @@ def test_python_refusals():
         pr.grouped_product(A, B, torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError, match="2-dimensional"):
         pr.dense_product(np.zeros((4, 5)), B)
+    with pytest.raises(ValueError, match="negated"):
+        pr.dense_product(torch.zeros(4, 5, dtype=torch.complex128).conj().imag, B)
 
 
 def test_predict_refusals():

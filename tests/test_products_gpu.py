@@ -457,3 +457,80 @@ def test_a_run_together(pr):
     new = rng.normal(size=(1, k))
     got = pr.dense_product(dev(new, torch.float64), bt[2], bias=b0t[2], act="logistic")
     np.testing.assert_allclose(host(got), expit(new @ beta[2] + b0[2]), rtol=1e-11)
+
+
+@pytest.mark.parametrize("cfg", [(0, 0), (16, 2), (64, 2), (128, 1)])
+def test_factors_and_result_as_blocks_of_one_matrix(pr, cfg):
+    rng = np.random.default_rng(9)
+    m, k, n = 37, 130, 21
+    big = dev(rng.normal(size=(m, k + n + 3)), torch.float64)
+    kept, B = big.clone(), dev(rng.normal(size=(k, n)), torch.float64)
+    A, C = big[:, :k], big[:, k + 1:k + 1 + n]
+    want = pr.dense_product(A, B, residual=C.clone(), cfg=cfg)
+    pr.dense_product(A, B, residual=C, out=C, cfg=cfg)
+    assert torch.equal(C, want)
+    kept[:, k + 1:k + 1 + n] = want
+    assert torch.equal(big, kept)
+    with pytest.raises(Exception, match="shares memory"):
+        pr.dense_product(A, B, out=big[:, k - 1:k - 1 + n], cfg=cfg)
+
+
+@pytest.mark.parametrize("need_A", [False, True])
+def test_more_runs_and_parts_than_a_grid_axis(pr, need_A):
+    """3000 runs, each asked to be cut into 32 parts."""
+    rng = np.random.default_rng(10)
+    gr, m, k, n = 3000, 7000, 3, 2
+    off = np.sort(rng.integers(0, m + 1, size=gr + 1))
+    A, B, dC = rng.normal(size=(m, k)), rng.normal(size=(gr, k, n)), rng.normal(size=(m, n))
+    got = pr.grouped_product_grad(dev(dC, torch.float64), dev(A, torch.float64), dev(B, torch.float64),
+                                  torch.from_numpy(off).to("cuda:0"), need_A=need_A, need_bias=True, cfg=(64, 32))
+    dB, tB = np.zeros((gr, k, n)), np.full((gr, k, n), 1e-300)
+    for g, (lo, hi) in enumerate(zip(off, off[1:])):
+        r = grad_reference(dC[lo:hi], A[lo:hi], B[g], "identity", dC[lo:hi], 1.0, 2.0 ** -53)
+        dB[g], tB[g] = r[4], r[5] + 1e-300
+    close(got[1], dB, tB)
+
+
+def test_a_dense_gradient_ignores_the_fields_of_runs(pr):
+    from locus_amd import _lib
+    rng = np.random.default_rng(11)
+    m, k, n = 700, 20, 33
+    A, B, dC, pre = (dev(rng.normal(size=s), torch.float64) for s in ((m, k), (k, n), (m, n), (m, n)))
+    want = pr.dense_product_grad(dC, A, B, act="silu", pre=pre, bias_grad="column")
+    got = [torch.full_like(w, float("nan")) for w in want]
+    off = torch.tensor([3, 5, 9, 40, 60], device="cuda:0")
+    src = torch.full((m,), -1, device="cuda:0")
+    fields = (m, n, k, 0, pr.ACTS["silu"], 0, 0, 0, 0, 1.0, *pr._at(dC), *pr._at(pre), *pr._at(A), *pr._at(B), 0,
+              *(g.data_ptr() for g in got), 0, 4, off.data_ptr(), 7, src.data_ptr(), 5)
+    lib = _lib.lib()
+    pr._run(pr._GRAD_ARGS.pack, lib.locus_hip_product_grad_dev, lib.locus_hip_product_grad_workspace_bytes, fields, A.device)
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
+def test_two_threads_on_their_own_streams(pr):
+    import threading
+    rng = np.random.default_rng(12)
+    A, B = dev(rng.normal(size=(70, 2003)), torch.float64), dev(rng.normal(size=(2003, 65)), torch.float64)
+    off = torch.tensor([0, 11, 70], device="cuda:0")
+    Bg, dC = torch.stack([B, 2 * B]), dev(rng.normal(size=(70, 65)), torch.float64)
+    calls = [lambda: (pr.dense_product(A, B, act="gelu"), pr.grouped_product(A, Bg, off, cfg=(64, 2))),
+             lambda: pr.grouped_product_grad(dC, A, Bg, off, act="probit", pre=dC, need_bias=True)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(call, ref):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                if not all(torch.equal(g, w) for g, w in zip(call(), ref)):
+                    wrong.append(call)
+        side.synchronize()
+
+    threads = [threading.Thread(target=work, args=x) for x in zip(calls, want)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
