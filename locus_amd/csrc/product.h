@@ -162,20 +162,21 @@ __device__ __forceinline__ long uniform_long(long v)
 
 __device__ __forceinline__ int bounded(int64_t v, int rows) { return v < 0 ? 0 : (v > rows ? rows : (int)v); }
 
-// 64 offsets at a time, one per lane: the ordered offsets are a running maximum, the tiles before a
-// run a running sum.  Every wave does this for itself (no barrier); under 1 us for up to 64 runs,
-// against a launch of its own for a tile map.  `tile` counts tiles of `bm` rows over all runs in
-// order; bm = 0 looks the run of row `tile` up instead.  Where no run holds the tile: lo = the tiles there
-// are, hi = the end of the last run.
-__device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int rows, int tile, int bm)
-{
-    const int lane = threadIdx.x & 63;
-    int carry = bounded(offsets[0], rows);
-    int before = 0;                                    // tiles of the runs before this chunk
-    Run found = {-1, 0, 0};
-    for (int base = 0; base < groups; base += 64) {
-        const int g = base + lane;
-        int hi = g < groups ? bounded(offsets[g + 1], rows) : 0;
+// 64 runs at a time, one per lane: the ordered offsets are a running maximum, the tiles of `bm` rows before
+// a run a running sum.  Every wave does this for itself (no barrier); under 1 us for up to 64 runs, against
+// a launch of its own for a tile map.
+struct RunScan {
+    const int64_t* offsets;
+    int groups, rows, bm;
+    int carry, before;       // the end of the runs so far, their tiles
+    int lo, hi, excl, tiles; // this lane's run: its rows, the tiles before it, its own
+
+    __device__ __forceinline__ RunScan(const int64_t* o, int g, int r, int b)
+        : offsets(o), groups(g), rows(r), bm(b), carry(bounded(o[0], r)), before(0) {}
+    __device__ __forceinline__ void next(int base)
+    {
+        const int lane = threadIdx.x & 63, g = base + lane;
+        hi = g < groups ? bounded(offsets[g + 1], rows) : 0;
         hi = hi > carry ? hi : carry;
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
@@ -183,43 +184,87 @@ __device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int 
             if (lane >= s && o > hi) hi = o;
         }
         const int up = __shfl_up(hi, 1);
-        const int lo = lane == 0 ? carry : up;
-        bool mine;
-        int excl = 0;
-        if (bm) {
-            const int t = (hi - lo + bm - 1) / bm;
-            int incl = t;
+        lo = lane == 0 ? carry : up;
+        tiles = (hi - lo + bm - 1) / bm;
+        int incl = tiles;
 #pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const int o = __shfl_up(incl, s);
-                if (lane >= s) incl += o;
-            }
-            excl = before + incl - t;
-            mine = tile >= excl && tile < before + incl;
-            before += __shfl(incl, 63);
-        } else {
-            mine = tile >= lo && tile < hi;
+        for (int s = 1; s < 64; s <<= 1) {
+            const int o = __shfl_up(incl, s);
+            if (lane >= s) incl += o;
         }
-        const unsigned long long hit = __ballot(mine && g < groups);
-        if (hit) {
-            const int src = __ffsll((long long)hit) - 1;
-            found.g = base + src;
-            const int rlo = __shfl(lo, src), rhi = __shfl(hi, src);
-            const int t0 = bm ? rlo + (tile - __shfl(excl, src)) * bm : rlo;
-            found.lo = t0;
-            found.hi = bm && rhi - t0 > bm ? t0 + bm : rhi;
-            break;
-        }
-        carry = __shfl(hi, 63);
+        excl = before + incl - tiles;
+        before += __builtin_amdgcn_readlane(incl, 63);
+        carry = __builtin_amdgcn_readlane(hi, 63);
     }
-    if (found.g < 0) {
-        found.lo = before;
-        found.hi = carry;
+    // the rows of `tile` if one of the lanes' runs holds it, else g = -1
+    __device__ __forceinline__ Run pick(int base, int tile) const
+    {
+        const unsigned long long hit = __ballot(tile >= excl && tile < excl + tiles);
+        if (hit == 0) return {-1, 0, 0};
+        const int src = __ffsll((long long)hit) - 1;
+        const int t0 = __builtin_amdgcn_readlane(lo, src) + (tile - __builtin_amdgcn_readlane(excl, src)) * bm;
+        const int end = __builtin_amdgcn_readlane(hi, src);
+        return {base + src, t0, end - t0 > bm ? t0 + bm : end};
     }
-    found.g = __builtin_amdgcn_readfirstlane(found.g);
-    found.lo = __builtin_amdgcn_readfirstlane(found.lo);
-    found.hi = __builtin_amdgcn_readfirstlane(found.hi);
-    return found;
+};
+
+// The run and rows of `tile`, counted over all runs in order.  Where no run holds it: lo = the tiles there
+// are, hi = the end of the last run.
+__device__ __forceinline__ Run find_run(const int64_t* offsets, int groups, int rows, int tile, int bm)
+{
+    RunScan scan(offsets, groups, rows, bm);
+    for (int base = 0; base < groups; base += 64) {
+        scan.next(base);
+        const Run r = scan.pick(base, tile);
+        if (r.g >= 0) return r;
+    }
+    return {-1, scan.before, scan.carry};
+}
+
+// A workgroup's place: tile (bx, by) of slice bz.
+struct Place {
+    unsigned bx, by, bz;
+};
+
+// Workgroup `lin` of a grid of gx x gy x gz: its place in a list that is cut into a contiguous eighth per
+// XCD (workgroups go to the XCDs in turn by their number).
+struct XcdList {
+    unsigned start, share, at;    // this XCD's part, the workgroup's number in it
+    __device__ __forceinline__ XcdList(unsigned lin, unsigned total)
+    {
+        const unsigned xcd = lin & 7, rem = total & 7;
+        start = xcd * (total >> 3) + (xcd < rem ? xcd : rem);
+        share = (total >> 3) + (xcd < rem ? 1 : 0);
+        at = lin >> 3;
+    }
+};
+
+// The run, rows and place of workgroup `lin`, columns of tiles one after the other.  The grid has room for more
+// tiles than runs of these lengths fill; up to 256 runs the workgroups without one come last in every
+// XCD's list: where they lay between the others, the CUs that took them stayed behind (10 runs, 1000 x 5000 x 501
+// float64 in four slices 165 us, 133 like this).  With more runs that count would cost longer than it saves.
+__device__ __forceinline__ Run place_run(const int64_t* offsets, int groups, int rows, int bm, unsigned lin,
+                                         unsigned gx, unsigned gy, unsigned gz, Place& at)
+{
+    const XcdList all(lin, gx * gy * gz);
+    if (groups > 256) {
+        const unsigned w = all.start + all.at, t = w % (gx * gy);
+        at = {t % gx, t / gx, w / (gx * gy)};
+        return find_run(offsets, groups, rows, at.bx, bm);
+    }
+    RunScan scan(offsets, groups, rows, bm);
+    for (int base = 0; base < groups; base += 64) scan.next(base);
+    const unsigned nx = scan.before;                   // tiles there are
+    const XcdList list(lin, nx * gy * gz);
+    if (list.at >= list.share) {
+        const unsigned q = all.start - list.start + list.at - list.share, rest = gx - nx;
+        at = {nx + q % rest, q / rest % gy, q / rest / gy};
+        return {-1, (int)nx, scan.carry};
+    }
+    const unsigned w = list.start + list.at, t = w % (nx * gy);
+    at = {t % nx, t / nx, w / (nx * gy)};
+    if (groups <= 64) return scan.pick(0, at.bx);
+    return find_run(offsets, groups, rows, at.bx, bm);
 }
 
 // Rows [lo, hi) of one run by its number (the same ordered offsets).

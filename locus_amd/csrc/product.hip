@@ -2,6 +2,7 @@
 // (joining a split sum, the gradient before the activation, column and row sums) and the C entry
 // points locus_hip_product_* (include/locus_hip.h).
 #include <algorithm>
+#include <cmath>
 #include <initializer_list>
 #include <utility>
 
@@ -11,30 +12,41 @@ namespace locus {
 
 namespace {
 
+// v + x[0] + x[step] + .. + x[(count - 1) step] in this order, up to DEEP of them: all loads are under way before
+// the first is needed, also where there are fewer (they read the last one again).
+template <int DEEP, class T> __device__ __forceinline__ T add_up(T v, const T* x, long step, int count)
+{
+    T t[DEEP];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) t[u] = x[(u < count ? u : count - 1) * step];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) v += u < count ? t[u] : T(0);
+    return v;
+}
+template <class T> __device__ __forceinline__ T sum_of(const T* x, long step, int count)
+{
+    T v = T(0);
+    for (; count > 8; count -= 16, x += 16 * step) v = add_up<16>(v, x, step, count);
+    return count > 0 ? add_up<8>(v, x, step, count) : v;
+}
+
 // C from the partial products of a split sum, added in the order of the slices (the same result
 // every time).  Bound by reading them; one thread per element along the partials' contiguous index; in
-// ROWS a lane looks its row's run up for the bias.
+// ROWS a lane looks its row's run up for the bias.  (A 64-bit division takes as many instructions as the rest.)
 template <class T, int MODE>
 __global__ void __launch_bounds__(256) product_join_kernel(const ProductDesc p)
 {
-    auto join = [&](long bias0, long i, long j) {
-        const T* x = static_cast<const T*>(p.part) + i * p.part_m + j * p.part_n;
-        T v = T(0);
-#pragma unroll 8
-        for (int z = 0; z < p.nz; ++z) v += x[z * p.part_z];
-        epi_store<T>(p.epi, bias0, i, j, v);
-    };
     const long len = (long)p.m * p.n;
+    const bool by_column = MODE == PRODUCT_DENSE && p.part_m == 1;
+    const int fast = by_column ? p.m : p.n;              // the contiguous index's length
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < (len + 63) / 64 * 64; e += (long)gridDim.x * 256) {
-        if constexpr (MODE == PRODUCT_DENSE) {
-            if (e >= len) break;
-            if (p.part_m == 1) join(0, e % p.m, e / p.m);
-            else join(0, e / p.n, e % p.n);
-        } else {                                          // whole waves stay together for the lookup
-            const long i = e < len ? e / p.n : p.m - 1;
-            const int g = find_runs(p.offsets, p.groups, p.m, (int)i);
-            if (g >= 0 && e < len) join(g * p.sbias_g, i, e % p.n);
-        }
+        const long at = e < len ? e : len - 1;           // whole waves stay together for the lookup
+        const long slow = len >> 32 ? at / fast : (unsigned)at / (unsigned)fast;
+        const long i = by_column ? at - slow * fast : slow;
+        const long j = by_column ? slow : at - slow * fast;
+        const int g = MODE == PRODUCT_ROWS ? find_runs(p.offsets, p.groups, p.m, (int)i) : 0;
+        if (e < len && g >= 0)
+            epi_store<T>(p.epi, g * p.sbias_g, i, j, sum_of(static_cast<const T*>(p.part) + at, p.part_z, p.nz));
     }
 }
 
@@ -95,10 +107,7 @@ __global__ void __launch_bounds__(256) product_sums_join_kernel(const T* sums, i
 {
     const long e = (long)blockIdx.x * 256 + threadIdx.x;
     if (e >= len) return;
-    T v = T(0);
-#pragma unroll 8
-    for (int q = 0; q < parts; ++q) v += sums[q * len + e];
-    out[e] = v;
+    out[e] = sum_of(sums + e, len, parts);
 }
 
 // Sums of G's rows (the gradient of a bias per row), one wave per row.
@@ -175,7 +184,10 @@ Plan plan_product(const Want& w)
     for (int tw = 4; tw >= 2; tw -= 2) {
         if (w.cfg[0] >= 64 && w.cfg[0] != 32 * tw) continue;
         const long bm = 32 * tw;
-        const long mt = runs ? p.groups * ((long)(avg + bm - 1) / bm) : (M + bm - 1) / bm;
+        // runs: half a tile more for each run, and a standard deviation or two of that sum (a tile more than
+        // there are places costs a round)
+        const long mt = runs ? (long)((double)M / bm + 0.5 * p.groups + 0.5 * std::sqrt((double)p.groups) + 0.5)
+                             : (M + bm - 1) / bm;
         const long tiles = std::max<long>(mt, 1) * ((N + bm - 1) / bm) * copies;
         const long most = 65535 / copies;                              // runs x parts: a grid's third axis
         const long asked = std::min<long>(w.cfg[1], most);
