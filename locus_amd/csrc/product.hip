@@ -51,16 +51,16 @@ __global__ void __launch_bounds__(256) product_join_kernel(const ProductDesc p)
 }
 
 // G = dC act'(pre) and the sums of its columns, per run and part of a run: bound by reading dC and
-// pre and writing G.  64 columns x 16 rows at a time; sums[part][groups][n], or the column sums themselves where
-// there is one part.
-template <class T>
+// pre and writing G.  COLS columns x 1024 / COLS rows at a time; sums[part][groups][n], or the column sums
+// themselves where there is one part.  Fewer columns, down to a line of memory, where there are few workgroups.
+template <class T, int COLS>
 __global__ void __launch_bounds__(1024) product_slope_kernel(const locus_hip_product_grad_args a, T* G,
                                                              int parts, T* sums)
 {
-    constexpr int ROWS = 16;
-    __shared__ T red[ROWS][64];
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const long j = (long)blockIdx.x * 64 + tx;
+    constexpr int ROWS = 1024 / COLS;
+    __shared__ T red[ROWS][COLS];
+    const int tx = threadIdx.x % COLS, ty = threadIdx.x / COLS;
+    const long j = (long)blockIdx.x * COLS + tx;
     const int part = blockIdx.y, g = blockIdx.z;
     long lo = 0, hi = a.m;
     if (a.offsets) {
@@ -93,10 +93,18 @@ __global__ void __launch_bounds__(1024) product_slope_kernel(const locus_hip_pro
     if (sums == nullptr) return;
     red[ty][tx] = sum;
     __syncthreads();
+    if (ROWS > 16) {                                     // to 16 rows
+        if (ty < 16) {
+#pragma unroll
+            for (int q = 16; q < ROWS; q += 16) sum += red[ty + q][tx];
+            red[ty][tx] = sum;
+        }
+        __syncthreads();
+    }
     if (ty == 0 && j < a.n) {
         T v = red[0][tx];
 #pragma unroll
-        for (int q = 1; q < ROWS; ++q) v += red[q][tx];
+        for (int q = 1; q < 16; ++q) v += red[q][tx];
         sums[((long)part * gridDim.z + g) * a.n + j] = v;
     }
 }
@@ -417,16 +425,23 @@ Want want_product(const locus_hip_product_args& a)
 
 // ---- gradient ------------------------------------------------------------------------------------
 
-// Parts of a run whose G and column sums are taken side by side: about two workgroups (of 16 waves) per
-// CU.  A part has rows enough to be worth the launch that joins them: 16 waves do 256 rows without an
-// activation, 64 with one (a 16-row turn of a float64 slope takes 2 to 3 us on a CU) in its time.
-int slope_parts(const locus_hip_product_grad_args& a)
+// How product_slope_kernel is cut.  Columns of a workgroup: 64, or fewer, down to 128 bytes, while that leaves
+// CUs without one.  Then parts of a run, up to about two workgroups (of 16 waves) per CU.  A part has rows enough to be
+// worth the launch that joins them: 16 waves do 256 rows of 64 columns without an activation, 64 with one (a 16-row
+// turn of a float64 slope takes 2 to 3 us on a CU) in its time.
+struct SlopeCut {
+    int cols, parts;
+};
+SlopeCut slope_cut(const locus_hip_product_grad_args& a)
 {
-    const long blocks = ((a.n + 63) / 64) * std::max<long>(1, a.groups);
-    const long per = a.m / std::max<long>(1, a.groups);
-    const long least = a.act == LOCUS_HIP_ACT_IDENTITY ? 256 : 64;
-    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks), per / least);
-    return (int)std::max<long>(1, std::min<long>(want, 1024));
+    const long groups = std::max<long>(1, a.groups), least_cols = a.dtype == LOCUS_HIP_F64 ? 16 : 32;
+    SlopeCut c = {64, 1};
+    auto blocks = [&] { return (a.n + c.cols - 1) / c.cols * groups; };
+    while (c.cols > least_cols && blocks() < device_cus() && a.m * c.cols > groups * 1024) c.cols /= 2;
+    const long least = (a.act == LOCUS_HIP_ACT_IDENTITY ? 256 : 64) * 64 / c.cols;
+    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks()), a.m / groups / least);
+    c.parts = (int)std::max<long>(1, std::min<long>(want, 1024));
+    return c;
 }
 
 int check_grad(const locus_hip_product_grad_args* a)
@@ -472,7 +487,7 @@ locus_hip_product_grad_args own_fields(locus_hip_product_grad_args a)
 // What a gradient launches: workspace [G | column sums | partials of dA | partials of dB].
 struct Grad {
     bool own_g, slope;                 // G in the workspace; G or sums are asked for
-    int parts;
+    SlopeCut cut;
     Want da, db;
     Plan pa, pb;
     long g_bytes, s_bytes, a_bytes, b_bytes;
@@ -487,9 +502,9 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     const long s = a.dtype == LOCUS_HIP_F64 ? 8 : 4;
     r.own_g = act && !a.G;
     r.slope = act || a.col_sums;
-    r.parts = slope_parts(a);
+    r.cut = slope_cut(a);
     r.g_bytes = r.own_g ? up(a.m * a.n * s) : 0;
-    r.s_bytes = a.col_sums && r.parts > 1 ? up(r.parts * std::max<long>(1, a.groups) * a.n * s) : 0;
+    r.s_bytes = a.col_sums && r.cut.parts > 1 ? up(r.cut.parts * std::max<long>(1, a.groups) * a.n * s) : 0;
     // G is row-major m x n, for the identity dC as it is
     const long g_m = act ? a.n : a.sd_m, g_n = act ? 1 : a.sd_n;
     Want w = {};
@@ -543,13 +558,16 @@ template <class T> int run_grad(const locus_hip_product_grad_args& a, Grad& r, h
     T* sums = static_cast<T*>(r.s_bytes ? ws + r.g_bytes : a.col_sums);
     if (r.slope && a.n > 0) {
         const unsigned groups = (unsigned)std::max<long>(1, a.groups);
-        hipLaunchKernelGGL(product_slope_kernel<T>, dim3((unsigned)((a.n + 63) / 64), (unsigned)r.parts, groups), dim3(1024),
-                           0, st, a, G, r.parts, sums);
+        const dim3 grid((unsigned)((a.n + r.cut.cols - 1) / r.cut.cols), (unsigned)r.cut.parts, groups);
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(1024), 0, st, a, G, r.cut.parts, sums); };
+        if (r.cut.cols == 64) go(product_slope_kernel<T, 64>);
+        else if (r.cut.cols == 32) go(product_slope_kernel<T, 32>);
+        else go(product_slope_kernel<T, 16>);
         LOCUS_HIP_CHECK(hipGetLastError());
         if (r.s_bytes) {
             const long len = (long)groups * a.n;
             hipLaunchKernelGGL(product_sums_join_kernel<T>, dim3((unsigned)((len + 255) / 256)), dim3(256), 0, st, sums,
-                               r.parts, len, static_cast<T*>(a.col_sums));
+                               r.cut.parts, len, static_cast<T*>(a.col_sums));
             LOCUS_HIP_CHECK(hipGetLastError());
         }
     }
