@@ -184,7 +184,7 @@ Plan plan_product(const Want& w)
         pl.nz = pl.kchunk > 0 ? (int)((K + pl.kchunk - 1) / pl.kchunk) : 1;
         return pl;
     }
-    const double cu_rate = (w.f64 ? 75e6 : 150e6) / w.cus;     // flop per us
+    const double cu_rate = (w.f64 ? 75e6 : 150e6) / device_cus();   // flop per us
     // us a workgroup alone on its CU takes for a million elements of the activation
     const bool cdf = p.epi.act == LOCUS_HIP_ACT_PROBIT || p.epi.act == LOCUS_HIP_ACT_GELU;
     const double heavy = p.epi.act == LOCUS_HIP_ACT_IDENTITY ? 0.0 : (w.f64 ? (cdf ? 2200.0 : 1000.0) : 400.0);
