@@ -46,8 +46,7 @@ extern "C" {
                                        points of section 1 return without touching the caller's
                                        buffers.  The reference's sweep cannot fail half-way
                                        (src/coreLoop.cpp:36-52).  Serialise cluster sweeps per GPU. */
-#define LOCUS_HIP_EWORKSPACE (-5)   /* locus_hip_product_*: no workspace, or one too small; nothing was
-                                       launched                                                  */
+#define LOCUS_HIP_EWORKSPACE (-5)   /* locus_hip_product_*: workspace too small; nothing was launched */
 
 const char* locus_hip_last_error(void);
 int locus_hip_version(void);      /* 100 * major + minor */
@@ -324,8 +323,10 @@ typedef struct locus_hip_product_args {
     const int64_t* gather; int64_t a_rows;        /* [m] or NULL                                */
     void* workspace; int64_t workspace_bytes;
 } locus_hip_product_args;
-int locus_hip_product_dev(const locus_hip_product_args* args, void* stream);
-/* Bytes of workspace for that call (pointers are not looked at), or a negative error. */
+/* 0, or a negative error; where the call needs a workspace and args->workspace is NULL, the bytes it needs (> 0),
+ * and nothing is launched: most calls need none, so a caller tries first. */
+int64_t locus_hip_product_dev(const locus_hip_product_args* args, void* stream);
+/* Bytes of workspace for that call (of the pointers only which are NULL is looked at), or a negative error. */
 int64_t locus_hip_product_workspace_bytes(const locus_hip_product_args* args);
 
 /* The gradient of that call, for dC (m x n) and the Z it kept in pre (not read for the identity):
@@ -350,8 +351,8 @@ typedef struct locus_hip_product_grad_args {
     const int64_t* gather; int64_t a_rows;
     void* workspace; int64_t workspace_bytes;
 } locus_hip_product_grad_args;
-int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* stream);
-/* Bytes of workspace (of the pointers only which are NULL is looked at), or a negative error. */
+int64_t locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* stream);
+/* As above. */
 int64_t locus_hip_product_grad_workspace_bytes(const locus_hip_product_grad_args* args);
 
 /* Element-wise part of coreBatch / coreZBatch / coreProbitBatch on [p][d] planes

@@ -141,6 +141,7 @@ struct Plan {
     bool swap = false;   // C' = B' A' (n is the short side)
     int nz = 1;
     long kchunk = 0;
+    double us = 0, join_us = 0;   // what it is expected to take, and the joining launch
 };
 
 // One product: its operands and what is asked of the plan.
@@ -149,80 +150,109 @@ struct Want {
     int mode;
     bool f64;
     int cfg[2];
-    long cus;            // CUs it may count on
-    long few, large;     // up to so many rows (or columns) take the kernel for few rows, where the other
-                         // factor has so many elements
+    long cus, all_cus;   // CUs it may count on, and the device's
+    bool tiles_only;     // not the kernel for few rows
+    double host_us;      // what a call with a workspace and another launch takes on the host: no gain below that
 };
 
-// Which kernel, tile and split.  A CU holds 4 workgroups of tiles of 64, 2 of 128; what share of its rate
-// it reaches with 1, 2, .. of them was measured (2000 x 500 x 20 000, both types within 3 %), as were the
-// microseconds a round of workgroups takes beside its products, and a joining launch: its own and the
-// partials written and read at 4.5 TB/s.
+// Which kernel, tile and split: the quickest by the estimates below, whose constants are fitted to measurements: 350
+// products of 1 .. 4000 rows, 20 .. 20 000 covariates and 1 .. 10 000 columns, alone or in up to 100 runs, in 26
+// geometries each, replayed from a graph.  The estimate's choice took 2 to 3 % longer than the best of them in either
+// type (rows up to 48 by the kernel for few, the rest in tiles: 12 % longer).
+//   Joining a split sum: 2.4 us, and the partials written and read at 4.2 TB/s.  Called one by one, a workspace and
+// another launch cost the host more than that (host_us).
+//   Few rows: 5.1 us, 1.2 for every round of two workgroups a CU, C and what goes with it at 9 TB/s, and the longer of:
+// a wave's blocks of k, 0.36 us each, times the workgroups a CU has; what they read through L2 at 7.6 TB/s (by the
+// root of what the last round leaves idle longer).
+//   Tiles: a CU holds 4 workgroups of tiles of 64, 2 of 128; the share of its rate that it reaches with 1, 2, .. of
+// them (2000 x 500 x 20 000, both types within 3 %), at least 0.48 us for a K-tile; 3.5 us, 3.5 and 9 for every
+// round of workgroups, C and what goes with it at 9 TB/s.
+//   Runs: half a tile more for each of them than their rows fill, and for tiles of 64 and 128 a standard deviation
+// or two of that sum (a tile more than there are places costs a round).
 Plan plan_product(const Want& w)
 {
-    Plan pl;
+    static const short splits[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64};
+    Plan best;
+    double best_call = 1e300;
     const ProductDesc& p = w.p;
-    const long M = p.m, N = p.n, K = p.k, s = w.f64 ? 8 : 4, bk = w.f64 ? 16 : 32;
+    const long M = p.m, N = p.n, K = p.k, s = w.f64 ? 8 : 4;
     const bool runs = w.mode == PRODUCT_ROWS, sums = w.mode == PRODUCT_SUM;
-    const double avg = runs ? (double)M / p.groups : (double)M;
     const long copies = sums ? p.groups : 1, len = sums ? (K + copies - 1) / copies : K;   // a sum's length
-    pl.kchunk = K;
-    const long side = runs ? (long)avg : std::min(M, N);
-    if (!sums) pl.rows = w.cfg[0] ? w.cfg[0] == 16 : side <= w.few && (runs || std::max(M, N) * K >= w.large);
-    if (pl.rows) {
-        pl.swap = !runs && N < M;
-        const long m = pl.swap ? N : M, n = pl.swap ? M : N, kb = w.f64 ? 8 : 16;
-        const long rt = runs ? std::max<long>(1, std::min<long>(m, m / 16 + p.groups)) : (m + 15) / 16;
-        const long wgs = rt * ((n + 63) / 64);
-        // two workgroups a CU; a sum that one workgroup ends in 24 blocks of k a wave is not split (a launch to
-        // join costs as much), else a wave gets 8 at least, and the partials stay within a tenth of B
-        long nz = std::min<long>(2 * w.cus / wgs, K > 96 * kb ? K / (32 * kb) : 1);
-        nz = std::min<long>(nz, (long)(0.1 * K / (runs ? avg : (double)m)));
-        if (w.cfg[1]) nz = w.cfg[1];
-        nz = std::max<long>(1, std::min<long>(nz, 256));
-        pl.kchunk = ((K + nz - 1) / nz + 4 * kb - 1) / (4 * kb) * (4 * kb);
-        pl.nz = pl.kchunk > 0 ? (int)((K + pl.kchunk - 1) / pl.kchunk) : 1;
-        return pl;
-    }
-    const double cu_rate = (w.f64 ? 75e6 : 150e6) / device_cus();   // flop per us
+    auto offer = [&](Plan pl, double us) {
+        if (pl.nz > 1) pl.join_us = 2.4 + 2.0 * pl.nz * M * N * copies * s / 4.2e6;
+        pl.us = us + pl.join_us;
+        const double call = std::max(pl.us, pl.nz > 1 ? w.host_us : 0.0);
+        if (call < best_call || (call == best_call && pl.us < best.us)) {
+            best = pl;
+            best_call = call;
+        }
+    };
+    auto each_split = [&](long most, auto take) {
+        if (w.cfg[1]) return take(std::min<long>(w.cfg[1], 65535 / copies));     // runs x parts: a grid's third axis
+        for (const long nz : splits) {
+            if (nz > 1 && (nz > most || best_call <= w.host_us)) break;
+            take(nz);
+        }
+    };
+
     // us a workgroup alone on its CU takes for a million elements of the activation
     const bool cdf = p.epi.act == LOCUS_HIP_ACT_PROBIT || p.epi.act == LOCUS_HIP_ACT_GELU;
     const double heavy = p.epi.act == LOCUS_HIP_ACT_IDENTITY ? 0.0 : (w.f64 ? (cdf ? 2200.0 : 1000.0) : 400.0);
-    double best = 1e300;
+    const double mn = 1e-6 * M * N * copies, outs = s * mn * (1 + !!p.epi.res + !!p.epi.pre + (p.epi.sb_m && p.epi.sb_n));
+    const bool asked = w.cfg[0] == 16;
+    const long side = runs ? M / p.groups : std::min(M, N);
+    if (!sums && (asked || (!w.cfg[0] && !w.tiles_only && side <= 1024))) {
+        const bool swap = !runs && N < M;
+        const long m = swap ? N : M, n = swap ? M : N, kb = w.f64 ? 8 : 16;
+        const double rt = runs ? std::max(1.0, std::min<double>(m, m / 16.0 + 0.5 * p.groups)) : (double)((m + 15) / 16);
+        const double ct = (double)((n + 63) / 64), l2 = s * K * rt * (std::max(n, 16l) + 16 * ct) / 7.6e6;
+        each_split(std::min<long>(64, K / (4 * kb)), [&](long nz) {
+            Plan pl;
+            pl.rows = true;
+            pl.swap = swap;
+            pl.kchunk = ((K + nz - 1) / nz + 4 * kb - 1) / (4 * kb) * (4 * kb);
+            pl.nz = pl.kchunk > 0 ? (int)((K + pl.kchunk - 1) / pl.kchunk) : 1;
+            const double wgs = rt * ct * pl.nz;
+            const double even = std::ceil(wgs / w.cus) * w.cus / wgs;    // the CUs' share of the last round
+            offer(pl, 5.1 + std::max(pl.kchunk / (4 * kb) * 0.36 * std::ceil(wgs / w.cus), l2 * std::sqrt(even)) +
+                          1.2 * std::ceil(wgs / (2 * w.cus)) + outs / 9.0 +
+                          (pl.nz == 1 ? mn * heavy / (2 * w.cus) : 0.0));
+        });
+    }
+    if (asked && !sums) return best;
+
+    // (the plan's own time, 1 to 2 us, counts in small calls: no tiles where they cannot be quicker)
+    const long bk = w.f64 ? 16 : 32;
+    if (!w.cfg[0] && best_call <= std::min(7.0 + 0.48 * len / bk, w.host_us)) return best;
+    const double cu_rate = (w.f64 ? 75e6 : 150e6) / w.all_cus;   // flop per us
     for (int tw = 4; tw >= 2; tw -= 2) {
         if (w.cfg[0] >= 64 && w.cfg[0] != 32 * tw) continue;
         const long bm = 32 * tw;
-        // runs: half a tile more for each run, and a standard deviation or two of that sum (a tile more than
-        // there are places costs a round)
         const long mt = runs ? (long)((double)M / bm + 0.5 * p.groups + 0.5 * std::sqrt((double)p.groups) + 0.5)
                              : (M + bm - 1) / bm;
         const long tiles = std::max<long>(mt, 1) * ((N + bm - 1) / bm) * copies;
-        const long most = 65535 / copies;                              // runs x parts: a grid's third axis
-        const long asked = std::min<long>(w.cfg[1], most);
-        for (long nz = asked ? asked : 1; nz <= (asked ? asked : std::min<long>(32, most)); ++nz) {
-            const long chunk = ((len + nz - 1) / nz + bk - 1) / bk * bk;
-            if (!w.cfg[1] && nz > 1 && chunk < 4 * bk) break;
-            const long used = sums ? nz : (K > 0 ? (K + chunk - 1) / chunk : 1);
-            const long wgs = tiles * used, load = (wgs + w.cus - 1) / w.cus, slots = tw == 4 ? 2 : 4;
+        const long most = std::min<long>(std::min<long>(32, len / (4 * bk)), 65535 / copies);
+        each_split(most, [&](long nz) {
+            Plan pl;
+            pl.tw = tw;
+            pl.kchunk = ((len + nz - 1) / nz + bk - 1) / bk * bk;
+            pl.nz = sums ? (int)nz : (int)(K > 0 ? (K + pl.kchunk - 1) / pl.kchunk : 1);
+            const long wgs = tiles * pl.nz, load = (wgs + w.cus - 1) / w.cus, slots = tw == 4 ? 2 : 4;
             static const double share2[5] = {0, 0.67, 0.80, 0.86, 0.90}, share4[3] = {0, 0.86, 0.92};
             const double* share = tw == 4 ? share4 : share2;
-            const double one = 2.0 * bm * bm * chunk / cu_rate;          // a workgroup's products on its CU
+            const double one = 2.0 * bm * bm * pl.kchunk / cu_rate;      // a workgroup's products on its CU
             const long rest = load % slots;
-            double t = one * ((load - rest) / share[slots] + (rest ? rest / share[rest] : 0.0)) +
-                       (double)((load + slots - 1) / slots) * (tw == 4 ? 9.0 : 6.0);
+            const double rounds = (double)((load + slots - 1) / slots);
+            double t = 3.5 + rounds * (tw == 4 ? 9.0 : 3.5) + outs / 9.0 +
+                       std::max(one * ((load - rest) / share[slots] + (rest ? rest / share[rest] : 0.0)),
+                                0.48 * pl.kchunk / bk * rounds);
             // the element function: in the epilogue by a CU's workgroups, after a split by all CUs
             const double f = 1e-6 * bm * bm * heavy;
-            t += used == 1 ? f * std::max<double>(1.0, (double)wgs / w.cus / 2) : f * tiles / w.cus / 2;
-            if (used > 1) t += 4.0 + 2.0 * used * M * N * copies * s / 4.5e6;
-            if (t < best) {
-                best = t;
-                pl.tw = tw;
-                pl.nz = (int)used;
-                pl.kchunk = chunk;
-            }
-        }
+            t += pl.nz == 1 ? f * std::max<double>(1.0, (double)wgs / w.cus / 2) : f * tiles / w.cus / 2;
+            offer(pl, t);
+        });
     }
-    return pl;
+    return best;
 }
 
 long plan_bytes(const Want& w, const Plan& pl)
@@ -301,8 +331,12 @@ int check_common(const char* what, int64_t m, int64_t n, int64_t k, int dtype, i
     return 0;
 }
 
-int no_workspace(const char* fn)
+// 0: there is enough; else what the entry point returns.
+int64_t no_workspace(int64_t need, const void* ws, int64_t bytes, const char* fn)
 {
+    if (need == 0) return 0;
+    if (!ws) return need;
+    if (bytes >= need) return 0;
     set_error(std::string("workspace smaller than ") + fn);
     return LOCUS_HIP_EWORKSPACE;
 }
@@ -418,8 +452,8 @@ Want want_product(const locus_hip_product_args& a)
     w.mode = a.mode;
     w.f64 = a.dtype == LOCUS_HIP_F64;
     w.cfg[0] = a.cfg[0]; w.cfg[1] = a.cfg[1];
-    w.cus = device_cus();
-    w.few = 48;
+    w.cus = w.all_cus = device_cus();
+    w.host_us = 14.5;
     return w;
 }
 
@@ -432,14 +466,14 @@ Want want_product(const locus_hip_product_args& a)
 struct SlopeCut {
     int cols, parts;
 };
-SlopeCut slope_cut(const locus_hip_product_grad_args& a)
+SlopeCut slope_cut(const locus_hip_product_grad_args& a, long cus)
 {
     const long groups = std::max<long>(1, a.groups), least_cols = a.dtype == LOCUS_HIP_F64 ? 16 : 32;
     SlopeCut c = {64, 1};
     auto blocks = [&] { return (a.n + c.cols - 1) / c.cols * groups; };
-    while (c.cols > least_cols && blocks() < device_cus() && a.m * c.cols > groups * 1024) c.cols /= 2;
+    while (c.cols > least_cols && blocks() < cus && a.m * c.cols > groups * 1024) c.cols /= 2;
     const long least = (a.act == LOCUS_HIP_ACT_IDENTITY ? 256 : 64) * 64 / c.cols;
-    const long want = std::min<long>(2L * device_cus() / std::max<long>(1, blocks()), a.m / groups / least);
+    const long want = std::min<long>(2 * cus / std::max<long>(1, blocks()), a.m / groups / least);
     c.parts = (int)std::max<long>(1, std::min<long>(want, 1024));
     return c;
 }
@@ -486,6 +520,7 @@ locus_hip_product_grad_args own_fields(locus_hip_product_grad_args a)
 
 // What a gradient launches: workspace [G | column sums | partials of dA | partials of dB].
 struct Grad {
+    bool pair;                         // both products in one launch
     bool own_g, slope;                 // G in the workspace; G or sums are asked for
     SlopeCut cut;
     Want da, db;
@@ -493,6 +528,11 @@ struct Grad {
     long g_bytes, s_bytes, a_bytes, b_bytes;
     long all() const { return g_bytes + s_bytes + a_bytes + b_bytes; }
 };
+
+bool pairs(const ProductDesc& p, int mode, int tw, const ProductDesc& q, int qmode, int qtw, bool f64)
+{
+    return f64 ? product_pairs<double>(p, mode, tw, q, qmode, qtw) : product_pairs<float>(p, mode, tw, q, qmode, qtw);
+}
 
 Grad plan_grad(const locus_hip_product_grad_args& a)
 {
@@ -502,7 +542,8 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     const long s = a.dtype == LOCUS_HIP_F64 ? 8 : 4;
     r.own_g = act && !a.G;
     r.slope = act || a.col_sums;
-    r.cut = slope_cut(a);
+    const long cus = device_cus();
+    r.cut = slope_cut(a, cus);
     r.g_bytes = r.own_g ? up(a.m * a.n * s) : 0;
     r.s_bytes = a.col_sums && r.cut.parts > 1 ? up(r.cut.parts * std::max<long>(1, a.groups) * a.n * s) : 0;
     // G is row-major m x n, for the identity dC as it is
@@ -510,9 +551,8 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     Want w = {};
     w.f64 = a.dtype == LOCUS_HIP_F64;
     w.cfg[0] = a.cfg[0]; w.cfg[1] = a.cfg[1];
-    w.cus = a.dA && a.dB ? device_cus() / 2 : device_cus();
-    w.few = 16;
-    w.large = 1 << 19;   // below, the two products in one launch are quicker
+    w.cus = w.all_cus = cus;
+    w.host_us = 16.0;
     w.p.epi.alpha = a.alpha;
     if (runs) {
         w.p.groups = (int)a.groups;
@@ -540,10 +580,26 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     if (a.k * std::max<long>(1, a.groups) >= (1l << 31)) r.db.cfg[1] = 1;       // dB's rows are counted in 32 bits
     if (a.dA) r.pa = plan_product(r.da);
     if (a.dB) r.pb = plan_product(r.db);
-    if (a.dA && a.dB && !r.pa.rows && !r.pb.rows && r.pa.tw != r.pb.tw) {   // one launch wants one tile
-        r.da.cfg[0] = r.db.cfg[0] = 64;
-        r.pa = plan_product(r.da);
-        r.pb = plan_product(r.db);
+    if (a.dA && a.dB && a.cfg[0] != 16) {
+        // both in one launch, tiles of one size, each with half the CUs; or one after the other (the second
+        // launch comes about 4 us cheaper than the estimate of one alone)
+        Want da = r.da, db = r.db;
+        da.cus = db.cus = cus / 2;
+        da.tiles_only = db.tiles_only = true;
+        Plan pa = plan_product(da), pb = plan_product(db);
+        if (pa.tw != pb.tw) {
+            da.cfg[0] = db.cfg[0] = 64;
+            pa = plan_product(da);
+            pb = plan_product(db);
+        }
+        const double joins = pa.join_us + pb.join_us;
+        void* const some = &r;         // (where partials lie does not matter here)
+        if (std::max(pa.us - pa.join_us, pb.us - pb.join_us) + joins <= r.pa.us + r.pb.us - 4.0 &&
+            pairs(planned(da, pa, some), da.mode, pa.tw, planned(db, pb, some), db.mode, pb.tw, w.f64)) {
+            r.pair = true;
+            r.pa = pa;
+            r.pb = pb;
+        }
     }
     if (a.dA) r.a_bytes = up(plan_bytes(r.da, r.pa));
     if (a.dB) r.b_bytes = up(plan_bytes(r.db, r.pb));
@@ -581,13 +637,11 @@ template <class T> int run_grad(const locus_hip_product_grad_args& a, Grad& r, h
     void* const pa = ws + r.g_bytes + r.s_bytes;
     void* const pb = ws + r.g_bytes + r.s_bytes + r.a_bytes;
     const bool da = a.dA && a.m > 0 && a.k > 0, db = a.dB && a.k > 0 && a.n > 0;
-    if (da && db && !r.pa.rows && !r.pb.rows) {
+    if (da && db && r.pair) {
         const ProductDesc p = planned(r.da, r.pa, pa), q = planned(r.db, r.pb, pb);
-        if (product_pairs<T>(p, r.da.mode, r.pa.tw, q, r.db.mode, r.pb.tw)) {
-            int rc = launch_product_pair<T>(p, r.da.mode, q, r.pa.tw, st);
-            if (!rc) rc = join_product<T>(p, r.da.mode, st);
-            return rc ? rc : join_product<T>(q, r.db.mode, st);
-        }
+        int rc = launch_product_pair<T>(p, r.da.mode, q, r.pa.tw, st);
+        if (!rc) rc = join_product<T>(p, r.da.mode, st);
+        return rc ? rc : join_product<T>(q, r.db.mode, st);
     }
     if (da) {
         const int rc = run_product<T>(r.da, r.pa, pa, st);
@@ -611,7 +665,7 @@ int64_t locus_hip_product_workspace_bytes(const locus_hip_product_args* args)
     return args->m == 0 || args->n == 0 ? 0 : plan_bytes(w, plan_product(w));
 }
 
-int locus_hip_product_dev(const locus_hip_product_args* args, void* stream)
+int64_t locus_hip_product_dev(const locus_hip_product_args* args, void* stream)
 {
     int rc = check_product(args);
     if (rc) return rc;
@@ -624,7 +678,8 @@ int locus_hip_product_dev(const locus_hip_product_args* args, void* stream)
     if ((rc = check_spans(a))) return rc;
     const Want w = want_product(a);
     const Plan pl = plan_product(w);
-    if (plan_bytes(w, pl) > (a.workspace ? a.workspace_bytes : 0)) return no_workspace("locus_hip_product_workspace_bytes()");
+    const int64_t lack = no_workspace(plan_bytes(w, pl), a.workspace, a.workspace_bytes, "locus_hip_product_workspace_bytes()");
+    if (lack) return lack;
     return w.f64 ? run_product<double>(w, pl, a.workspace, (hipStream_t)stream)
                  : run_product<float>(w, pl, a.workspace, (hipStream_t)stream);
 }
@@ -635,7 +690,7 @@ int64_t locus_hip_product_grad_workspace_bytes(const locus_hip_product_grad_args
     return rc ? rc : plan_grad(own_fields(*args)).all();
 }
 
-int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* stream)
+int64_t locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* stream)
 {
     int rc = check_grad(args);
     if (rc) return rc;
@@ -649,7 +704,8 @@ int locus_hip_product_grad_dev(const locus_hip_product_grad_args* args, void* st
                   "product_grad: rows gathered from an empty matrix");
     if ((rc = check_grad_spans(a))) return rc;
     Grad r = plan_grad(a);
-    if (r.all() > (a.workspace ? a.workspace_bytes : 0)) return no_workspace("locus_hip_product_grad_workspace_bytes()");
+    const int64_t lack = no_workspace(r.all(), a.workspace, a.workspace_bytes, "locus_hip_product_grad_workspace_bytes()");
+    if (lack) return lack;
     return a.dtype == LOCUS_HIP_F64 ? run_grad<double>(a, r, (hipStream_t)stream) : run_grad<float>(a, r, (hipStream_t)stream);
 }
 

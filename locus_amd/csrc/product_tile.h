@@ -532,7 +532,8 @@ template <class T> int tile_layout(const ProductDesc& p, int mode, int tw)
     const bool off32 = p.sa_m >= 0 && p.sa_k >= 0 && p.sb_n >= 0 && p.sb_k >= 0 &&
                        (a_m - 1) * p.sa_m + (a_k - 1) * p.sa_k <= lim &&
                        (bm - 1) * p.sb_n + (BK - 1) * p.sb_k <= lim;
-    const bool ak = p.sa_k == 1, bk = p.sb_k == 1;
+    // (one column has no stride of its own: it goes with the layout of a pair and of sums over runs)
+    const bool ak = p.sa_k == 1, bk = p.sb_k == 1 && !(p.n == 1 && mode != PRODUCT_ROWS && !ak);
     if (!off32 || (mode == PRODUCT_ROWS && !ak) || (mode == PRODUCT_SUM && (bk || (ak && !p.gather)))) return LAY_ANY;
     if (mode == PRODUCT_SUM) return LAY_FAST | (p.gather ? LAY_GATHER : 0);
     return LAY_FAST | (ak ? LAY_A_K : 0) | (bk ? LAY_B_K : 0);

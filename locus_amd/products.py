@@ -29,7 +29,6 @@ from . import _lib
 ACTS = {"identity": 0, "logistic": 1, "probit": 2, "softplus": 3, "gelu": 4, "silu": 5}
 _DTYPES = {torch.float64: 0, torch.float32: 1}
 _DENSE, _ROWS = 0, 1
-_EWORKSPACE = -5                                 # LOCUS_HIP_EWORKSPACE
 _ARGS = struct.Struct("=3q6i2d26q")              # struct locus_hip_product_args
 _GRAD_ARGS = struct.Struct("=3q6id24q")          # struct locus_hip_product_grad_args
 
@@ -104,25 +103,23 @@ def _index(name, t, like, size):
         _fail(f"{name} must be contiguous")
 
 
-def _run(pack, run_fn, need_fn, fields, dev):
+def _run(pack, run, fields, dev):
     """One call of the library on the current stream of `dev`: `fields` of the argument struct up to the
     workspace, which is made when the library asks for one."""
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _run(pack, run_fn, need_fn, fields, dev)
+            return _run(pack, run, fields, dev)
     stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    rc = run_fn(pack(*fields, 0, 0), stream)
-    if rc == _EWORKSPACE:
-        need = need_fn(pack(*fields, 0, 0))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = run_fn(pack(*fields, ws.data_ptr(), need), stream)
+    rc = run(pack(*fields, 0, 0), stream)
+    if rc > 0:
+        ws = torch.empty(rc, dtype=torch.uint8, device=dev)
+        rc = run(pack(*fields, ws.data_ptr(), rc), stream)
     if rc:
         _lib.check(rc)
 
 
 def _forward(fields, dev):
-    lib = _lib.lib()
-    _run(_ARGS.pack, lib.locus_hip_product_dev, lib.locus_hip_product_workspace_bytes, fields, dev)
+    _run(_ARGS.pack, _lib.lib().locus_hip_product_dev, fields, dev)
 
 
 def _at(t):
@@ -220,8 +217,7 @@ def _gradient(dC, A, B, dtype, act, pre, alpha, need_A, need_B, bias_grad, m, n,
     elif bias_grad == "matrix" and code:
         G = A.new_empty((m, n))
     sb = B.stride()
-    lib = _lib.lib()
-    _run(_GRAD_ARGS.pack, lib.locus_hip_product_grad_dev, lib.locus_hip_product_grad_workspace_bytes,
+    _run(_GRAD_ARGS.pack, _lib.lib().locus_hip_product_grad_dev,
          (m, n, k, dtype, code, _ROWS if groups else _DENSE, 0, *cfg, alpha, *_at(dC), *_at(pre if code else None),
           *_at(A), B.data_ptr(), sb[-2], sb[-1], _ptr(G), _ptr(dA), _ptr(dB), _ptr(cols), _ptr(rows), groups,
           _ptr(offsets), sb[0] if groups else 0, _ptr(gather), A.shape[0]), A.device)

@@ -69,21 +69,24 @@ def test_null_arguments_and_missing_workspace(monkeypatch):
     split = dict(m=64, n=64, k=4096, sa_m=4096, sb_k=64, sc_m=64, B=16 << 20, C=32 << 20, cfg0=64, cfg1=4)
     need = lib.locus_hip_product_workspace_bytes(args(**split))
     assert need == 4 * 64 * 64 * 8
-    assert lib.locus_hip_product_dev(args(**split), None) == EWORKSPACE
+    assert lib.locus_hip_product_dev(args(**split), None) == need            # what to bring, nothing launched
     assert lib.locus_hip_product_dev(args(**split, workspace=64 << 20, workspace_bytes=need - 1), None) == EWORKSPACE
     g = dict(act=1, pre=6 << 20, sp_m=3, sp_n=1)
-    assert lib.locus_hip_product_grad_workspace_bytes(grad(**g)) >= 4 * 3 * 8
-    assert lib.locus_hip_product_grad_dev(grad(**g), None) == EWORKSPACE
+    need = lib.locus_hip_product_grad_workspace_bytes(grad(**g))
+    assert need >= 4 * 3 * 8
+    assert lib.locus_hip_product_grad_dev(grad(**g), None) == need
+    assert lib.locus_hip_product_grad_dev(grad(**g, workspace=64 << 20, workspace_bytes=need - 1), None) == EWORKSPACE
 
 
 @pytest.mark.parametrize("at,ok", [(512, True), (504, False), (1000, True), (1008, False), (1016, False), (1024, False),
                                    (1536, True), (2024, True), (-24, True), (-16, False), (-1024 + 512, True)])
 def test_blocks_of_one_matrix_share_no_memory(monkeypatch, at, ok):
     """A: columns 0 .. 63 of rows of 128 (1024 bytes), C: 3 other columns `at` bytes from there, or not quite.  (The
-    missing workspace stops the calls that pass.)"""
+    small workspace stops the calls that pass.)"""
     monkeypatch.setenv("LOCUS_HIP_MFMA_CUS", "256")
     lib = _lib.lib()
-    rc = lib.locus_hip_product_dev(args(m=4, n=3, k=64, sa_m=128, sc_m=128, C=(1 << 20) + at, cfg0=64, cfg1=4), None)
+    rc = lib.locus_hip_product_dev(args(m=4, n=3, k=64, sa_m=128, sc_m=128, C=(1 << 20) + at, cfg0=64, cfg1=4,
+                                        workspace=64 << 20, workspace_bytes=1), None)
     assert rc == (EWORKSPACE if ok else EINVAL)
 
 

@@ -502,8 +502,7 @@ def test_a_dense_gradient_ignores_the_fields_of_runs(pr):
     src = torch.full((m,), -1, device="cuda:0")
     fields = (m, n, k, 0, pr.ACTS["silu"], 0, 0, 0, 0, 1.0, *pr._at(dC), *pr._at(pre), *pr._at(A), *pr._at(B), 0,
               *(g.data_ptr() for g in got), 0, 4, off.data_ptr(), 7, src.data_ptr(), 5)
-    lib = _lib.lib()
-    pr._run(pr._GRAD_ARGS.pack, lib.locus_hip_product_grad_dev, lib.locus_hip_product_grad_workspace_bytes, fields, A.device)
+    pr._run(pr._GRAD_ARGS.pack, _lib.lib().locus_hip_product_grad_dev, fields, A.device)
     for g, w in zip(got, want):
         assert torch.equal(g, w)
 
