@@ -1,8 +1,9 @@
 // Matrix product of few rows (tiles of 16) with the epilogue of ProductEpi: one new sample against all
-// effects, a served batch, runs of a few rows each.  B is read once (per tile of rows) and bounds the
-// time; the matrix cores take the products whatever the number of rows.  (Tiles of 32 and 64 rows
-// that load B once for all of them are no faster: 33 samples x 20 011 x 1000 float32 33 us with three tiles
-// of 16, whose second and third reading of B comes from L2, 37 and 35 with the larger ones.)
+// effects, a served batch, runs of a few rows each, and whatever is small.  B is read once (per tile of rows) and
+// bounds the time: one row x 20 000 x 1000 float64 28 us (160 MB, 5.6 TB/s), 70 rows in 64 runs x 2000 x 200 float32
+// 22 us (102 MB, 4.7 TB/s).  The matrix cores take the products whatever the number of rows.  (Tiles of 32 and 64
+// rows that load B once for all of them are no faster: 33 samples x 20 011 x 1000 float32 33 us with three tiles of
+// 16, whose second and third reading of B comes from L2, 37 and 35 with the larger ones.)
 //
 // A workgroup of four waves owns 16 rows x 64 columns and a slice of k; its waves take a quarter
 // of the slice each and are added through LDS, the slices by product_join_kernel (or, where there is

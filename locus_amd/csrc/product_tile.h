@@ -2,24 +2,30 @@
 // float64 or float32).
 //
 // A workgroup of four waves (2 x 2) owns a BM x BN = (32 TW) x (32 TW) tile of C, a wave TW x TW
-// matrix-core tiles of it.  K-tiles of BK travel global memory -> registers -> LDS, two buffers, one
-// barrier per K-tile: tile t + 1 goes to LDS and tile t + 2 is requested before the products of
-// tile t.  With TW = 4 a wave does 64 matrix instructions per K-tile (4096 cycles) against 32 LDS reads
-// and 16 + 16 single-element moves, and two workgroups share a CU (74 KB of LDS each), so that one's
-// barrier hides behind the other's products.  LDS rows are 17 elements longer than the tile: odd, so
-// that the transposing stores of an operand whose contiguous index is k spread over the banks.
+// matrix-core tiles of it.  K-tiles of BK = 16 (float64) or 32 travel global memory -> registers -> LDS, two
+// buffers, one barrier per K-tile.  The work is cut into steps of four k: a step first reads the operands
+// of the next one, then moves its share of the coming K-tiles (t + 1 to LDS, t + 1 + PF from memory), then
+// does its TW x TW matrix instructions, so that they wait for no read just issued.  LDS rows are 15 elements
+// longer than the tile: odd, so that the transposing stores of an operand whose contiguous index is k spread
+// over the banks, and small enough that tiles of 64 (40 KB) fit a CU four times, tiles of 128 (74 KB) twice.
+// Those four keep its matrix cores 90 % busy (2000 x 20 000 x 500 float64; 79 % in the two products of a gradient,
+// 1999 x 5000 x 1000 float32); one alone reaches 67 % of the rate.  Tiles of 128 read half as much and are chosen
+// where the sums are long and the tiles fill the chip evenly.
 //
 // The K loop does no vector address arithmetic: an element is a raw buffer load from a scalar base
-// (advanced on the scalar unit) plus a loop-invariant 32-bit lane offset.  On gfx950 vector
-// instructions take issue time from the matrix instructions of the same SIMD.  OFF32 = false is the
-// same with 64-bit lane addresses, for tiles that reach over 2^31 bytes and for gathered rows.
+// (advanced on the scalar unit) plus a loop-invariant 32-bit lane offset, one instruction for any alignment.
+// On gfx950 vector instructions take issue time from the matrix instructions of the same SIMD.  LAY_ANY is the
+// same with 64-bit lane addresses, for tiles that reach over 2^31 bytes, negative strides and layouts that no
+// caller of weight has.
 //
 // Rows and columns beyond the matrix read the tile's first one (they feed only elements that are
-// never stored); only a last, partial K-tile checks k.
+// never stored); only the last K-tiles check k, and steps beyond the end are skipped.
 //
-// Epilogue: the accumulators pass through LDS (the tile buffers are free then), half the tile's rows
-// at a time, so that the element function is compiled once in a rolled loop and bias, residual, the
-// kept Z and C are read and written along C's contiguous index, whichever it is.
+// Epilogue: the accumulators pass through LDS (the tile buffers are free then), all the tile's rows at a time or
+// half of them, so that the element function is compiled once in a rolled loop and bias, residual, the
+// kept Z and C are read and written along C's contiguous index, whichever it is.  Bound by memory where sums are
+// short: 1000 x 63 x 10 000 float64 with its residual, 160 MB, takes 49 us (3.3 TB/s; it was 120 with an address
+// computed for each element).
 #pragma once
 #include <type_traits>
 
@@ -518,8 +524,8 @@ __global__ void __launch_bounds__(256, TW == 4 ? 2 : 4) product_pair_kernel(cons
     }
 }
 
-// The form a product takes: FAST and its layout, or LAY_ANY.  Compiled fast: every layout of one matrix pair;
-// runs of rows with A contiguous along a row; sums over runs with both operands contiguous along theirs.
+// The form a product takes: FAST and its layout, or LAY_ANY.  Compiled fast: every layout of one matrix pair and of
+// runs of rows; sums over runs with B contiguous along a row, and a gathered A, too.
 template <class T> int tile_layout(const ProductDesc& p, int mode, int tw)
 {
     constexpr int BK = tile_bk<T>();
@@ -534,8 +540,8 @@ template <class T> int tile_layout(const ProductDesc& p, int mode, int tw)
                        (bm - 1) * p.sb_n + (BK - 1) * p.sb_k <= lim;
     // (one column has no stride of its own: it goes with the layout of a pair and of sums over runs)
     const bool ak = p.sa_k == 1, bk = p.sb_k == 1 && !(p.n == 1 && mode != PRODUCT_ROWS && !ak);
-    if (!off32 || (mode == PRODUCT_ROWS && !ak) || (mode == PRODUCT_SUM && (bk || (ak && !p.gather)))) return LAY_ANY;
-    if (mode == PRODUCT_SUM) return LAY_FAST | (p.gather ? LAY_GATHER : 0);
+    if (!off32 || (mode == PRODUCT_SUM && bk)) return LAY_ANY;
+    if (mode == PRODUCT_SUM && p.gather) return LAY_FAST | LAY_GATHER;
     return LAY_FAST | (ak ? LAY_A_K : 0) | (bk ? LAY_B_K : 0);
 }
 
@@ -563,9 +569,12 @@ int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
             else go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, LAY_FAST>);
         } else if (mode == PRODUCT_ROWS) {
             if (lay == (AK | BK)) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK | BK>);
-            else go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK>);
+            else if (lay == AK) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK>);
+            else if (lay == BK) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, BK>);
+            else go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, LAY_FAST>);
         } else {
             if (p.gather) go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST | LAY_GATHER>);
+            else if (lay == AK) go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, AK>);
             else go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST>);
         }
     };
@@ -582,7 +591,8 @@ int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
     return 0;
 }
 
-// Pairs that are compiled: a gradient's two products of row-major operands, dA = G B' and dB = A' G.
+// Pairs that are compiled: a gradient's two products of row-major G and B, dA = G B' and dB = A' G, with A row-major,
+// column-major or gathered by rows.
 template <class T>
 bool product_pairs(const ProductDesc& p, int mode, int tw, const ProductDesc& q, int qmode, int qtw)
 {
@@ -590,7 +600,7 @@ bool product_pairs(const ProductDesc& p, int mode, int tw, const ProductDesc& q,
     const TileGrid g = tile_grid(p, mode, 32 * tw), h = tile_grid(q, qmode, 32 * tw);
     const double all = (double)g.x * g.y * g.z + (double)h.x * h.y * h.z;
     return tw == qtw && all < (1 << 23) && (mode == PRODUCT_DENSE ? qmode == PRODUCT_DENSE : mode == PRODUCT_ROWS && qmode == PRODUCT_SUM) &&
-           tile_layout<T>(p, mode, tw) == ABK && (tile_layout<T>(q, qmode, tw) & ~LAY_GATHER) == LAY_FAST;
+           tile_layout<T>(p, mode, tw) == ABK && (tile_layout<T>(q, qmode, tw) & ~LAY_GATHER & ~LAY_A_K) == LAY_FAST;
 }
 
 template <class T>
@@ -603,7 +613,11 @@ int launch_product_pair(const ProductDesc& p, int mode, const ProductDesc& q, in
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, d); };
     auto pick = [&](auto twc) {
         constexpr int TW = decltype(twc)::value;
-        if (mode == PRODUCT_DENSE) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>);
+        constexpr int AK = LAY_FAST | LAY_A_K;
+        const bool by_column = tile_layout<T>(q, qmode, tw) & LAY_A_K;
+        if (mode == PRODUCT_DENSE && by_column) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK, PRODUCT_DENSE, AK>);
+        else if (mode == PRODUCT_DENSE) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>);
+        else if (by_column) go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, AK>);
         else if (q.gather) go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST | LAY_GATHER>);
         else go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST>);
     };
