@@ -533,3 +533,48 @@ def test_two_threads_on_their_own_streams(pr):
     for th in threads:
         th.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("groups", [64, 65, 256, 257, 700])
+@pytest.mark.parametrize("cfg", [(0, 0), (16, 1), (64, 1), (64, 2), (128, 1)])
+def test_many_runs(pr, groups, cfg):
+    """Around the numbers of runs at which a tile's run is looked up in another way."""
+    rng = np.random.default_rng(groups)
+    m, k, n = 2500, 37, 66
+    off = np.sort(rng.integers(3, m - 4, size=groups + 1))
+    A, B, dC = rng.normal(size=(m, k)), rng.normal(size=(groups, k, n)), rng.normal(size=(m, n))
+    want, tol = np.zeros((m, n)), np.zeros((m, n))
+    dA, tA = np.zeros((m, k)), np.zeros((m, k))
+    dB, tB = np.zeros((groups, k, n)), np.full((groups, k, n), 1e-300)
+    for g, (lo, hi) in enumerate(zip(off, off[1:])):
+        _, _, want[lo:hi], tol[lo:hi] = reference(A[lo:hi], B[g], None, "identity", None, 1.0, 0.0, 2.0 ** -53, k)
+        _, _, dA[lo:hi], tA[lo:hi], dB[g], t, *_ = grad_reference(dC[lo:hi], A[lo:hi], B[g], "identity", dC[lo:hi], 1.0, 2.0 ** -53)
+        tB[g] += t
+    args = dev(A, torch.float64), dev(B, torch.float64), torch.from_numpy(off).to("cuda:0")
+    close(pr.grouped_product(*args, cfg=cfg), want, tol)
+    ga, gb, _ = pr.grouped_product_grad(dev(dC, torch.float64), *args, cfg=cfg)
+    close(ga, dA, tA)
+    close(gb, dB, tB)
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32"])
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("cfg", [(0, 0), (64, 1), (64, 3), (128, 1)])
+def test_gradients_of_one_and_two_columns(pr, dtype, n, cfg):
+    t = DT[dtype]
+    u = torch.finfo(t).eps / 2
+    for m, k, lay in ((300, 203, "row"), (300, 203, "col"), (33, 1500, "win")):
+        rng = np.random.default_rng(m + n)
+        f32 = lambda *s: rng.normal(size=s).astype(np.float32).astype(np.float64)  # noqa: E731
+        A, B, dC, pre = f32(m, k), f32(k, n), f32(m, n), 2 * f32(m, n)
+        for act in ("identity", "logistic"):
+            r = grad_reference(dC, A, B, act, pre, 1.0, u)
+            for runs in (False, True):
+                off = torch.tensor([0, m], device="cuda:0")
+                args = [layout(dC, lay, t), layout(A, lay, t), layout(B, lay, t)]
+                args = args if not runs else [args[0], args[1], args[2][None], off]
+                fn = pr.grouped_product_grad if runs else pr.dense_product_grad
+                got = fn(*args, act=act, pre=layout(pre, lay, t), cfg=cfg, **(dict(need_bias=True) if runs else dict(bias_grad="column")))
+                close(got[0], r[2], r[3] + 1e-300)
+                close(got[1][0] if runs else got[1], r[4], r[5] + 1e-300)
+                close(got[2][0] if runs else got[2], r[6], r[7])
