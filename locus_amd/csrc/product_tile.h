@@ -56,8 +56,8 @@ __device__ __forceinline__ T buffer_elem(const char* base, unsigned off, unsigne
 // elements along C's contiguous index per thread and turn, addresses stepped, not multiplied out (a
 // 64-bit product per element and matrix made short sums cost 26 us where writing C takes 8).  Partial
 // products and act = identity go U turns at a time, their residuals loaded first; the other functions
-// take long enough to hide one load.
-template <class T, int HM, int BN, int EL>
+// take long enough to hide one load.  PLAIN: C = alpha sum and no more (gradients: half the code).
+template <class T, int HM, int BN, int EL, bool PLAIN>
 __device__ __forceinline__ void store_block(const ProductDesc& p, const T* lds, bool mfast, long m0, int n0,
                                             int rows, int cols, long bias0, long c0, unsigned bz, bool gr,
                                             bool outside)
@@ -72,8 +72,8 @@ __device__ __forceinline__ void store_block(const ProductDesc& p, const T* lds, 
     const bool whole = cnt >= VE;
     const ProductEpi& e = p.epi;
     const bool raw = p.part != nullptr;
-    const int act = raw ? LOCUS_HIP_ACT_IDENTITY : e.act;
-    const bool has_res = !raw && e.res, has_pre = !raw && e.pre, has_bias = !raw && e.bias;
+    const int act = PLAIN || raw ? LOCUS_HIP_ACT_IDENTITY : e.act;
+    const bool has_res = !PLAIN && !raw && e.res, has_pre = !PLAIN && !raw && e.pre, has_bias = !PLAIN && !raw && e.bias;
     const long gi = m0 + (mfast ? f0 : s0), gj = n0 + (mfast ? s0 : f0);
     auto walk = [&](const void* base, long off, long sm, long sn) {
         return static_cast<T*>(const_cast<void*>(base)) + off + gi * sm + gj * sn;
@@ -177,7 +177,8 @@ __device__ __forceinline__ void store_block(const ProductDesc& p, const T* lds, 
 
 // How a kernel is compiled for the operands: FAST with each operand's contiguous index (k or not),
 // or the general form: run-time layouts and 64-bit lane addresses.
-enum { LAY_ANY = 0, LAY_FAST = 1, LAY_A_K = 2, LAY_B_K = 4, LAY_GATHER = 8 /* a fast sum's gathered A */ };
+enum { LAY_ANY = 0, LAY_FAST = 1, LAY_A_K = 2, LAY_B_K = 4, LAY_GATHER = 8 /* a fast sum's gathered A */,
+       LAY_PLAIN = 16 /* with FAST: nothing but alpha in the epilogue */ };
 
 // Workgroup `lin` of a grid of gx x gy x gz.
 template <class T, int TW, int BK, int PF, int MODE, int LAY>
@@ -321,10 +322,13 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
     // asks for an offset outside the buffer resource, which the hardware answers with 0 (no branches in
     // short sums).  Gathered sums: one row of A per wave and element; lane q holds the q-th one of the
     // K-tile (rows), read a K-tile ahead.
+    bool outside = false;               // a gathered row outside A: the run's C is NaN
     auto gathered = [&](int k0) -> int {
         if (MODE != PRODUCT_SUM || !gs) return 0;
         const int k = k0 + ak0 + lane % NQ * QM;
-        return (int)in_a(p.gather[k < kEnd ? k : kb]);
+        const long row = p.gather[k < kEnd ? k : kb];
+        outside |= row < 0 || row >= p.a_rows;
+        return (int)in_a(row);
     };
     auto get_a = [&](int q, int rows, bool in) -> T {
         if (MODE == PRODUCT_SUM && gs) {
@@ -458,13 +462,9 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
         }
     }
 
-    // A gathered sum over a row outside A: its run's C is NaN.
-    bool outside = false;
-    if (gs) {
-        for (int k = kb + tid; k < kEnd; k += 256) outside |= p.gather[k] < 0 || p.gather[k] >= p.a_rows;
-        outside = __syncthreads_or(outside);
-    }
+    if (gs) outside = __syncthreads_or(outside);
 
+    constexpr bool PLAIN = MODE == PRODUCT_SUM || (LAY & LAY_PLAIN) != 0;
     // Through LDS, all rows at a time or half of them, then along C's contiguous index.
     constexpr int HALVES = BM * (BN + 1) <= G::ELEMS ? 1 : 2, HM = BM / HALVES, EL = BN + 1;
     const bool mfast = p.part ? p.part_m == 1 : (p.epi.sc_n != 1 && p.epi.sc_m == 1);
@@ -482,7 +482,7 @@ __device__ __forceinline__ void product_tile(const ProductDesc& p, T* lds, unsig
         }
         __syncthreads();
         const int rows = (int)(mEnd - m0 - h * HM < HM ? mEnd - m0 - h * HM : HM);
-        store_block<T, HM, BN, EL>(p, lds, mfast, m0 + h * HM, n0, rows, nCols, bias0, c0, bz, gr, outside);
+        store_block<T, HM, BN, EL, PLAIN>(p, lds, mfast, m0 + h * HM, n0, rows, nCols, bias0, c0, bz, gr, outside);
         if (h + 1 < HALVES) __syncthreads();
     }
 }
@@ -613,13 +613,13 @@ int launch_product_pair(const ProductDesc& p, int mode, const ProductDesc& q, in
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, d); };
     auto pick = [&](auto twc) {
         constexpr int TW = decltype(twc)::value;
-        constexpr int AK = LAY_FAST | LAY_A_K;
+        constexpr int PL = LAY_PLAIN, AK = LAY_FAST | LAY_A_K;
         const bool by_column = tile_layout<T>(q, qmode, tw) & LAY_A_K;
-        if (mode == PRODUCT_DENSE && by_column) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK, PRODUCT_DENSE, AK>);
-        else if (mode == PRODUCT_DENSE) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK, PRODUCT_DENSE, LAY_FAST>);
-        else if (by_column) go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, AK>);
-        else if (q.gather) go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST | LAY_GATHER>);
-        else go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK, PRODUCT_SUM, LAY_FAST>);
+        if (mode == PRODUCT_DENSE && by_column) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK | PL, PRODUCT_DENSE, AK | PL>);
+        else if (mode == PRODUCT_DENSE) go(product_pair_kernel<T, TW, PRODUCT_DENSE, ABK | PL, PRODUCT_DENSE, LAY_FAST | PL>);
+        else if (by_column) go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK | PL, PRODUCT_SUM, AK>);
+        else if (q.gather) go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK | PL, PRODUCT_SUM, LAY_FAST | LAY_GATHER>);
+        else go(product_pair_kernel<T, TW, PRODUCT_ROWS, ABK | PL, PRODUCT_SUM, LAY_FAST>);
     };
     if (tw == 2) pick(std::integral_constant<int, 2>{});
     else pick(std::integral_constant<int, 4>{});
