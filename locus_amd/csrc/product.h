@@ -21,6 +21,9 @@ struct ProductEpi {
     int act;
 };
 
+// C = alpha sum and no more.
+inline bool epi_plain(const ProductEpi& e) { return !e.bias && !e.res && !e.pre && e.act == LOCUS_HIP_ACT_IDENTITY; }
+
 // Modes of a product: one pair of matrices; runs of rows with a B of their own; runs of the summed
 // index with a C of their own (the gradient of the runs' B).
 enum { PRODUCT_DENSE = 0, PRODUCT_ROWS = 1, PRODUCT_SUM = 2 };

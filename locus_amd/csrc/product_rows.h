@@ -34,7 +34,8 @@ template <class T> struct Vec16 {
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-template <class T, int BKIND, int MODE>
+// PLAIN: partial products, or C = alpha sum and no more.
+template <class T, int BKIND, int MODE, bool PLAIN>
 __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
 {
     constexpr int V = Vec16<T>::V;
@@ -226,6 +227,8 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const ProductDesc p)
             }
             if (p.part)
                 static_cast<T*>(p.part)[blockIdx.z * p.part_z + gi * p.part_m + gj * p.part_n] = v;
+            else if (PLAIN)
+                static_cast<T*>(p.epi.C)[gi * p.epi.sc_m + gj * p.epi.sc_n] = T(p.epi.alpha) * v;
             else
                 epi_store<T>(p.epi, bias0, gi, gj, v);
         }
@@ -241,11 +244,15 @@ int launch_product_rows(const ProductDesc& p, int mode, hipStream_t st)
                                               : run_tiles(p, 16);
     const int kind = p.sb_n == 1 && p.n >= V ? ROWS_BK_N : (p.sb_k == 1 ? ROWS_BK_K : ROWS_BK_ANY);
     const bool dense = mode == PRODUCT_DENSE;
+    const bool plain = p.part || epi_plain(p.epi);
+    const dim3 grid(dense ? gx : gy, dense ? gy : gx, (unsigned)p.nz);
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, p); };
     auto pick = [&](auto kc) {
         constexpr int KIND = decltype(kc)::value;
-        const dim3 grid(dense ? gx : gy, dense ? gy : gx, (unsigned)p.nz);
-        if (dense) hipLaunchKernelGGL((product_rows_kernel<T, KIND, PRODUCT_DENSE>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((product_rows_kernel<T, KIND, PRODUCT_ROWS>), grid, dim3(256), 0, st, p);
+        if (dense && plain) go(product_rows_kernel<T, KIND, PRODUCT_DENSE, true>);
+        else if (dense) go(product_rows_kernel<T, KIND, PRODUCT_DENSE, false>);
+        else if (plain) go(product_rows_kernel<T, KIND, PRODUCT_ROWS, true>);
+        else go(product_rows_kernel<T, KIND, PRODUCT_ROWS, false>);
     };
     if (kind == ROWS_BK_N) pick(std::integral_constant<int, ROWS_BK_N>{});
     else if (kind == ROWS_BK_K) pick(std::integral_constant<int, ROWS_BK_K>{});

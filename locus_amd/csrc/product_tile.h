@@ -556,25 +556,28 @@ inline TileGrid tile_grid(const ProductDesc& p, int mode, int bm)
 template <class T>
 int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
 {
-    const int lay = tile_layout<T>(p, mode, tw);
+    // partial products and plain ones by kernels without the rest of the epilogue
+    const bool plain = mode == PRODUCT_SUM || p.part || epi_plain(p.epi);
+    const int form = tile_layout<T>(p, mode, tw), lay = form && plain ? form | LAY_PLAIN : form;
     const TileGrid g = tile_grid(p, mode, lay ? 32 * tw : 64);
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(g.x, g.y, g.z), dim3(256), 0, st, p); };
-    auto pick = [&](auto twc) {
-        constexpr int TW = decltype(twc)::value, PF = TW == 2 ? 2 : 1;
-        constexpr int AK = LAY_FAST | LAY_A_K, BK = LAY_FAST | LAY_B_K;
+    auto pick = [&](auto twc, auto plc) {
+        constexpr int TW = decltype(twc)::value, PF = TW == 2 ? 2 : 1, PL = decltype(plc)::value;
+        constexpr int AK = LAY_FAST | LAY_A_K | PL, BK = LAY_FAST | LAY_B_K | PL, NONE = LAY_FAST | PL;
         if (mode == PRODUCT_DENSE) {
             if (lay == (AK | BK)) go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, AK | BK>);
             else if (lay == AK) go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, AK>);
             else if (lay == BK) go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, BK>);
-            else go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, LAY_FAST>);
+            else go(product_tile_kernel<T, TW, PF, PRODUCT_DENSE, NONE>);
         } else if (mode == PRODUCT_ROWS) {
             if (lay == (AK | BK)) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK | BK>);
             else if (lay == AK) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, AK>);
             else if (lay == BK) go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, BK>);
-            else go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, LAY_FAST>);
-        } else {
+            else go(product_tile_kernel<T, TW, PF, PRODUCT_ROWS, NONE>);
+        } else if constexpr (PL != 0) {
+            constexpr int AK = LAY_FAST | LAY_A_K;
             if (p.gather) go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST | LAY_GATHER>);
-            else if (lay == AK) go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, AK>);
+            else if (form == AK) go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, AK>);
             else go(product_tile_kernel<T, TW, PF, PRODUCT_SUM, LAY_FAST>);
         }
     };
@@ -582,10 +585,13 @@ int launch_product_tile(const ProductDesc& p, int mode, int tw, hipStream_t st)
         if (mode == PRODUCT_DENSE) go(product_tile_kernel<T, 2, 1, PRODUCT_DENSE, LAY_ANY>);
         else if (mode == PRODUCT_ROWS) go(product_tile_kernel<T, 2, 1, PRODUCT_ROWS, LAY_ANY>);
         else go(product_tile_kernel<T, 2, 1, PRODUCT_SUM, LAY_ANY>);
-    } else if (tw == 4) {
-        pick(std::integral_constant<int, 4>{});
     } else {
-        pick(std::integral_constant<int, 2>{});
+        const auto pl = std::integral_constant<int, LAY_PLAIN>{};
+        const auto full = std::integral_constant<int, 0>{};
+        if (tw == 4 && plain) pick(std::integral_constant<int, 4>{}, pl);
+        else if (tw == 4) pick(std::integral_constant<int, 4>{}, full);
+        else if (plain) pick(std::integral_constant<int, 2>{}, pl);
+        else pick(std::integral_constant<int, 2>{}, full);
     }
     LOCUS_HIP_CHECK(hipGetLastError());
     return 0;
