@@ -578,3 +578,23 @@ def test_gradients_of_one_and_two_columns(pr, dtype, n, cfg):
                 close(got[0], r[2], r[3] + 1e-300)
                 close(got[1][0] if runs else got[1], r[4], r[5] + 1e-300)
                 close(got[2][0] if runs else got[2], r[6], r[7])
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32"])
+@pytest.mark.parametrize("m,k,n", [(17, 333, 8300), (1, 700, 64), (16, 64, 4099), (33, 1030, 130), (5, 5000, 3)])
+@pytest.mark.parametrize("layb", ["row", "col", "win"])
+def test_few_rows_long_and_wide(pr, dtype, m, k, n, layb):
+    """The kernel for few rows, whole and in slices, on every layout of B, up to 130 workgroups side by side."""
+    t = DT[dtype]
+    u = torch.finfo(t).eps / 2
+    rng = np.random.default_rng(m + k)
+    A = rng.normal(size=(m, k)).astype(np.float32).astype(np.float64)
+    B = rng.normal(size=(k, n)).astype(np.float32).astype(np.float64)
+    bias = rng.normal(size=(1, n)).astype(np.float32).astype(np.float64)
+    for act, b, cfg in (("identity", None, (16, 1)), ("softplus", bias, (16, 1)), ("logistic", bias, (16, 3)), ("silu", bias, (0, 0))):
+        _, _, want, tol = reference(A, B, b, act, None, 1.0, 0.0, u, k)
+        got = pr.dense_product(dev(A, t), layout(B, layb, t), bias=None if b is None else dev(b, t), act=act, cfg=cfg)
+        close(got, want, tol)
+        off = torch.tensor([0, m], device="cuda:0")
+        got = pr.grouped_product(dev(A, t), layout(B, layb, t)[None], off, bias=None if b is None else dev(b, t), act=act, cfg=cfg)
+        close(got, want, tol)
