@@ -459,10 +459,10 @@ Want want_product(const locus_hip_product_args& a)
 
 // ---- gradient ------------------------------------------------------------------------------------
 
-// How product_slope_kernel is cut.  Columns of a workgroup: 64, or fewer, down to 128 bytes, while that leaves
-// CUs without one.  Then parts of a run, up to about two workgroups (of 16 waves) per CU.  A part has rows enough to be
-// worth the launch that joins them: 16 waves do 256 rows of 64 columns without an activation, 64 with one (a 16-row
-// turn of a float64 slope takes 2 to 3 us on a CU) in its time.
+// How product_slope_kernel is cut.  Columns of a workgroup (of 16 waves): 64, or fewer, down to 128 bytes, while all
+// workgroups run side by side, one on a CU in float64 (94 registers), two in float32.  Then parts of a run, up to two
+// workgroups per CU.  A part has rows enough to be worth the launch that joins them: 16 waves do 256 rows of 64 columns without an
+// activation, 64 with one (a 16-row turn of a float64 slope takes 2 to 3 us on a CU) in its time.
 struct SlopeCut {
     int cols, parts;
 };
@@ -471,7 +471,8 @@ SlopeCut slope_cut(const locus_hip_product_grad_args& a, long cus)
     const long groups = std::max<long>(1, a.groups), least_cols = a.dtype == LOCUS_HIP_F64 ? 16 : 32;
     SlopeCut c = {64, 1};
     auto blocks = [&] { return (a.n + c.cols - 1) / c.cols * groups; };
-    while (c.cols > least_cols && blocks() < cus && a.m * c.cols > groups * 1024) c.cols /= 2;
+    const long room = a.dtype == LOCUS_HIP_F64 ? cus : 2 * cus;
+    while (c.cols > least_cols && 2 * blocks() <= room && a.m * c.cols > groups * 1024) c.cols /= 2;
     const long least = (a.act == LOCUS_HIP_ACT_IDENTITY ? 256 : 64) * 64 / c.cols;
     const long want = std::min<long>(2 * cus / std::max<long>(1, blocks()), a.m / groups / least);
     c.parts = (int)std::max<long>(1, std::min<long>(want, 1024));
