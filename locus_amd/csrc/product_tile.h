@@ -547,9 +547,9 @@ template <class T> int tile_layout(const ProductDesc& p, int mode, int tw)
 {
     constexpr int BK = tile_bk<T>();
     const int bm = 32 * tw;
-    // 32-bit lane offsets: a K-tile's elements lie within 2^31 bytes behind its first one (a gathered
-    // A: all of A does)
-    const long lim = ((1L << 31) - 1) / (long)sizeof(T);
+    // 32-bit lane offsets: a K-tile's elements lie, whole, within the 2^31 - 1 bytes of buffer_elem's window behind its
+    // first one (a gathered A: all of A does); of one that ended at 2^31 the hardware would make a 0
+    const long lim = ((1L << 31) - 1) / (long)sizeof(T) - 1;
     const long a_m = mode == PRODUCT_ROWS && p.gather ? p.a_rows : bm;
     const long a_k = mode == PRODUCT_SUM && p.gather ? p.a_rows : BK;
     const bool off32 = p.sa_m >= 0 && p.sa_k >= 0 && p.sb_n >= 0 && p.sb_k >= 0 &&
