@@ -297,7 +297,7 @@ template <int TWM, int TWN, int KS, int BK>
 static int launch_gemm(const GemmDesc& g, dim3 grid, hipStream_t st)
 {
     constexpr int BM = 32 * TWM, BN = 32 * TWN;
-    const long lim = (1L << 28) - 1;  // elements
+    const long lim = (1L << 28) - 2;  // elements: the last one ends within the window's 2^31 - 1 bytes
     const bool off32 = !getenv("LOCUS_HIP_GEMM_OFF64") && g.sa_m >= 0 && g.sa_k >= 0 &&
                        g.sb_n >= 0 && g.sb_k >= 0 &&
                        (BM - 1) * g.sa_m + (BK - 1) * g.sa_k <= lim &&

@@ -50,3 +50,22 @@ def test_last_element_of_two_gigabytes(pr, big, dtype, step, cfg):
         dA, dB, _ = pr.grouped_product_grad(dC, A, other[None], off, gather=gather, cfg=cfg)
         same(dB[0], P, S)
     same(pr.dense_product_grad(dC, A, other, cfg=cfg)[1], P, S)
+
+
+@pytest.mark.parametrize("step", [-1, 0, 1])
+def test_last_element_of_two_gigabytes_plain_product(hip, big, monkeypatch, step):
+    """The same for locus_hip_gemm_dev (K-tiles of 16, rows of A and columns of B)."""
+    from locus_amd import device as dv
+    monkeypatch.setenv("LOCUS_HIP_GEMM_BK", "16")
+    rng = np.random.default_rng(step + 5)
+    far = 4260880 + step
+    A = big.as_strided((64, 16), (far, 1))
+    A.copy_(torch.from_numpy(rng.normal(size=(64, 16))))
+    other = torch.from_numpy(rng.normal(size=(16, 70))).to("cuda:0")
+    P, S = A.contiguous() @ other, A.contiguous().abs() @ other.abs()
+    C = torch.empty((64, 70), dtype=torch.float64, device="cuda:0")
+    dv.gemm(64, 70, 16, A, far, 1, other, 70, 1, C, 70, 1)
+    assert ((C - P).abs() <= 2 * 82 * 2.0 ** -53 * S).all()
+    C = torch.empty((70, 64), dtype=torch.float64, device="cuda:0")
+    dv.gemm(70, 64, 16, other, 1, 70, A, 1, far, C, 64, 1)
+    assert ((C - P.t()).abs() <= 2 * 82 * 2.0 ** -53 * S.t()).all()
