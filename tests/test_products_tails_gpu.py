@@ -68,3 +68,29 @@ def test_values(pr, act, dtype, cfg):
     got = pr.dense_product(col, torch.ones((1, 1), dtype=t, device="cuda:0"), act=act, cfg=cfg)[:, 0].cpu().double()
     want = [value_and_slope(act, x)[0] for x in z]
     check(got.numpy(), want, [abs(v) for v in want], z, 16, torch.finfo(t).eps / 2, f"{act} {dtype} value")
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32"])
+@pytest.mark.parametrize("act", ACTS)
+def test_slopes(pr, act, dtype):
+    t = DT[dtype]
+    z = points(dtype, act)
+    col = torch.from_numpy(z[:, None]).to("cuda:0").to(t)
+    got = pr.dense_product_grad(torch.ones_like(col), col, torch.ones((1, 1), dtype=t, device="cuda:0"), act=act, pre=col,
+                                need_A=False, need_B=False, bias_grad="matrix")[2][:, 0].cpu().double()
+    want = [value_and_slope(act, x) for x in z]
+    check(got.numpy(), [w[1] for w in want], [w[2] for w in want], z, 24, torch.finfo(t).eps / 2, f"{act} {dtype} slope")
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32"])
+@pytest.mark.parametrize("act", ["probit", "gelu"])
+def test_slopes_of_huge_values(pr, act, dtype):
+    """Whose squares overflow: 0 on both sides, gelu's 1 on the right; NaN stays."""
+    t = DT[dtype]
+    far = torch.finfo(t).max
+    col = torch.tensor([[39.0], [41.0], [1e10], [far / 2], [far], [float("inf")]], dtype=t, device="cuda:0")
+    col = torch.cat([col, -col, col.new_full((1, 1), float("nan"))])
+    got = pr.dense_product_grad(torch.ones_like(col), col, col.new_ones((1, 1)), act=act, pre=col, need_A=False,
+                                need_B=False, bias_grad="matrix")[2][:, 0].cpu().double().numpy()
+    right = got[:6] - (1.0 if act == "gelu" else 0.0)
+    assert np.abs(right).max() <= 1e-300 and np.abs(got[6:12]).max() <= 1e-300 and np.isnan(got[12])
