@@ -68,9 +68,9 @@ template <class T> __device__ __forceinline__ T logistic(T z)
 
 // Phi(z).  The tail at a = |z| is exp(-a^2 / 2) erfcx(x) / 2 with x = a / sqrt 2, and (1 + 2 x) erfcx(x) is a
 // polynomial in t = (x - 3.75) / (x + 3.75) (Shepherd and Laframboise, Math. Comp. 36, 1981): degree 23
-// truncates at 5e-17; its coefficients were computed here with 60 digits.  a^2 / 2 is carried with its
-// rounding error.  At most 8 units of rounding relative (2e4 points against 25 digits), from -38 up;
-// below 0.
+// truncates at 5.1e-17; its coefficients were computed with 60 digits (scripts/microbench/cdf_poly.py).  a^2 / 2 is
+// carried with its rounding error.  At most 8 units of rounding relative from -37.5 up; below, where results are no
+// longer normal numbers, within one of the smallest positive number more; 0 from -38.6 down.
 static __device__ const double kCdfPoly[24] = {
     0x1.3ccda0b5d5dc2p+0, -0x1.1f367683f89a5p-3, 0x1.d5f294816277ep-9, 0x1.510169d09665bp-4,
     -0x1.bda9309a35871p-4, 0x1.7a14188a9ce2ap-4, -0x1.e0d0fa6c16f3fp-5, 0x1.d0b0037d167adp-6,

@@ -94,3 +94,16 @@ def test_slopes_of_huge_values(pr, act, dtype):
                                 need_B=False, bias_grad="matrix")[2][:, 0].cpu().double().numpy()
     right = got[:6] - (1.0 if act == "gelu" else 0.0)
     assert np.abs(right).max() <= 1e-300 and np.abs(got[6:12]).max() <= 1e-300 and np.isnan(got[12])
+
+
+def test_values_below_the_normal_numbers(pr):
+    """Phi in float64 from -37.5 down, 2^-1022 and less: 8 units relative, and half of 2^-1074 each for the last product
+    and the exponential before it, which is larger than the result by 90 and rounded to the same grid at worst."""
+    rng = np.random.default_rng(0)
+    z = np.concatenate([-rng.uniform(37.4, 38.7, 400), [-38.48, -38.6, -39.0, -40.0, -1e3]])
+    col = torch.from_numpy(z[:, None]).to("cuda:0")
+    got = pr.dense_product(col, col.new_ones((1, 1)), act="probit")[:, 0].cpu().numpy()
+    with mp.workdps(40):
+        for zi, g in zip(z, got):
+            v = mp.ncdf(mp.mpf(zi))
+            assert abs(mp.mpf(float(g)) - v) <= 8 * mp.mpf(2) ** -53 * v + mp.mpf(2) ** -1074, zi
