@@ -23,15 +23,20 @@ def _matrix(name, a, cols=None):
 
 def _raw_effects(eff, A, rmvd):
     """Effects on standardised columns -> effects on the raw ones and the constant they leave:
-    ((A - m) / s) e = A (e / s) - m' (e / s); removed columns have effect 0."""
+    ((A - m) / s) e = A (e / s) - m' (e / s); removed columns have effect 0.  Means and deviations as scale_rm_ takes
+    them, over all columns: sums over some would round otherwise.  A column of one value that is not a binary fraction
+    (0.1, say) may have been kept there, its rounded mean a little off and its deviation no more than that: standardised
+    it is constant, so what it adds is a constant, whatever a new sample holds."""
     keep = np.setdiff1d(np.arange(A.shape[1]), rmvd if rmvd is not None else [])
     if eff.shape[0] != len(keep):
         raise ValueError("the training covariates do not go with the fit: "
                          f"{len(keep)} columns kept, {eff.shape[0]} rows of effects")
-    mean, sd = A[:, keep].mean(axis=0), A[:, keep].std(axis=0, ddof=1)
+    mean, sd = A.mean(axis=0)[keep], A.std(axis=0, ddof=1)[keep]
+    flat = (A.max(axis=0) == A.min(axis=0))[keep]
+    const = ((A[0, keep] - mean) / sd)[flat] @ eff[flat]
     out = np.zeros((A.shape[1], eff.shape[1]))
-    out[keep] = eff / sd[:, None]
-    return out, -(mean @ out[keep])
+    out[keep[~flat]] = eff[~flat] / sd[~flat, None]
+    return out, const - mean @ out[keep]
 
 
 class Predictor:

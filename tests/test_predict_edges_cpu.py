@@ -1,0 +1,27 @@
+"""The folding of the standardisation into the effects (locus_amd.predict), without a GPU."""
+import numpy as np
+import pytest
+
+
+@pytest.mark.parametrize("order", ["C", "F"])
+@pytest.mark.parametrize("value", [0.1, 0.3, 1 / 3, 1e-3, 7.7, 2.0, 0.0, 1e9 + 0.1])
+def test_columns_of_one_value(order, value):
+    """Such a column is kept by scale_rm_ where its rounded mean is off.  Terms of order 1 (raw columns of order 1),
+    sums of 6 of them, twice: 1e-13 holds them with room."""
+    from locus_amd.predict import _raw_effects
+    from locus_amd.prepare import scale_rm_
+    kept = 0
+    for n in range(20, 120, 3):
+        rng = np.random.default_rng(n)
+        X = np.array(rng.normal(size=(n, 6)), order=order)
+        X[:, 2] = value
+        Xs, rmvd = scale_rm_(X)
+        kept += not rmvd[2]
+        eff = rng.normal(size=(Xs.shape[1], 2))
+        out, const = _raw_effects(eff, X, np.nonzero(rmvd)[0])
+        assert np.abs(X @ out + const - Xs @ eff).max() <= 1e-13
+        new = rng.normal(size=(4, 6))                  # of another value there: the same constant
+        same = new.copy()
+        same[:, 2] = value
+        assert np.abs((new - same) @ out).max() == 0
+    assert kept or value in (2.0, 0.0)
