@@ -105,13 +105,14 @@ class Predictor:
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.dtype = torch.float32 if single else torch.float64
         up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self.device, self.dtype)  # noqa: E731
-        self.parts = [(act, cols, up(np.stack([e[:, cols] for e in effects])), up(np.stack([c[cols] for c in consts])))
-                      for act, cols in parts if len(cols)]
+        self.parts = [(act, torch.from_numpy(cols).to(self.device), up(np.stack([e[:, cols] for e in effects])),
+                       up(np.stack([c[cols] for c in consts]))) for act, cols in parts if len(cols)]
 
     def score(self, A, fit=None, type="response"):
         """Device-side form: A is a GPU tensor (samples x (p + q), raw covariates, those of Z behind those
         of X) of the predictor's type; returns a GPU tensor (samples x d) and does not wait for it.
-        fit: which fit scores each sample (0-based integers, on the host), for a predictor of many."""
+        fit: which fit scores each sample (0-based integers, on the host), for a predictor of many.  Without it the
+        call can be captured into a HIP graph; with it, it cannot: the order of the samples is made on the host."""
         import torch
         from . import products
         if type not in ("response", "link"):
@@ -126,11 +127,15 @@ class Predictor:
             fit = np.asarray(fit)
             if fit.shape != (n,) or fit.dtype.kind not in "iu" or (n and not (0 <= fit.min() and fit.max() < groups)):
                 raise ValueError(f"fit must hold {n} integers from 0 to {groups - 1}")
-            host = np.argsort(fit, kind="stable")
-            order = torch.from_numpy(host).to(self.device)
-            off = torch.from_numpy(np.searchsorted(fit[host], np.arange(groups + 1)).astype(np.int64)).to(self.device)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("score() with fit cannot be captured into a graph: a replay would not see a new fit")
+            order = np.argsort(fit, kind="stable")
+            off = np.searchsorted(fit[order], np.arange(groups + 1))
+            host = torch.empty(n + groups + 1, dtype=torch.int64, pin_memory=True)    # (a copy from other memory waits)
+            host.numpy()[:] = np.concatenate([order, off])
+            order, off = host.to(self.device, non_blocking=True).split([n, groups + 1])
         out = torch.empty((n, self.d), dtype=self.dtype, device=self.device)
-        for act, cols, B, const in self.parts:
+        for act, at, B, const in self.parts:
             act = act if type == "response" else "identity"
             if fit is None:
                 part = products.dense_product(A, B[0], bias=const[0], act=act)
@@ -141,8 +146,7 @@ class Predictor:
             if len(self.parts) == 1:
                 out[order] = part
             else:
-                at = torch.from_numpy(cols).to(self.device)
-                out[(order[:, None] if fit is not None else torch.arange(n, device=self.device)[:, None]), at] = part
+                out[order[:, None] if fit is not None else slice(None), at] = part
         return out
 
     def __call__(self, X_new, Z_new=None, fit=None, type="response"):
