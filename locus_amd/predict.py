@@ -102,7 +102,9 @@ class Predictor:
         import torch
         from . import device as dv
         dv.require_gpu()
-        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.device = torch.device("cuda" if device is None else device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.dtype = torch.float32 if single else torch.float64
         up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self.device, self.dtype)  # noqa: E731
         self.parts = [(act, torch.from_numpy(cols).to(self.device), up(np.stack([e[:, cols] for e in effects])),

@@ -77,3 +77,12 @@ def test_captured_and_replayed(hip, link):
         A + 1
         with pytest.raises(RuntimeError, match="captured"):
             many.score(A, np.arange(33) % 2)
+
+
+def test_device_without_a_number_is_the_current_one(hip):
+    """"cuda" names whatever device is current when it is looked at: the predictor fixes it where its effects are."""
+    from locus_amd import Predictor
+    vb, X = fits(1)
+    for device in (None, "cuda", "cuda:0", torch.device("cuda")):
+        pred = Predictor(vb[0], X[0], link="probit", device=device)
+        assert pred.device == pred.parts[0][2].device == torch.device("cuda", torch.cuda.current_device())
