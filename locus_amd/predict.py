@@ -127,6 +127,8 @@ class Predictor:
         order = off = None
         if fit is not None:
             fit = np.asarray(fit)
+            if fit.size == 0:                                     # (numpy takes an empty list for floats)
+                fit = fit.astype(np.int64)
             if fit.shape != (n,) or fit.dtype.kind not in "iu" or (n and not (0 <= fit.min() and fit.max() < groups)):
                 raise ValueError(f"fit must hold {n} integers from 0 to {groups - 1}")
             if torch.cuda.is_current_stream_capturing():

@@ -86,3 +86,14 @@ def test_device_without_a_number_is_the_current_one(hip):
     for device in (None, "cuda", "cuda:0", torch.device("cuda")):
         pred = Predictor(vb[0], X[0], link="probit", device=device)
         assert pred.device == pred.parts[0][2].device == torch.device("cuda", torch.cuda.current_device())
+
+
+@pytest.mark.parametrize("link", ["probit", "mix"])
+@pytest.mark.parametrize("fit", [[], (), np.array([], dtype=int), np.array([])], ids=["list", "tuple", "int", "float"])
+def test_no_samples(hip, link, fit):
+    from locus_amd import Predictor
+    vb, X = fits(2)
+    pred = Predictor(vb, X, link=link, ind_bin=[1] if link == "mix" else None)
+    assert pred(np.zeros((0, 9)), fit=fit).shape == (0, 6)
+    with pytest.raises(ValueError, match="integers"):
+        pred(np.zeros((1, 9)), fit=fit)
