@@ -452,7 +452,7 @@ Want want_product(const locus_hip_product_args& a)
     w.mode = a.mode;
     w.f64 = a.dtype == LOCUS_HIP_F64;
     w.cfg[0] = a.cfg[0]; w.cfg[1] = a.cfg[1];
-    w.cus = w.all_cus = device_cus();
+    w.cus = w.all_cus = real_cus();          // (LOCUS_HIP_MFMA_CUS is for the sweeps' launch plan)
     w.host_us = 14.5;
     return w;
 }
@@ -543,7 +543,7 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
     const long s = a.dtype == LOCUS_HIP_F64 ? 8 : 4;
     r.own_g = act && !a.G;
     r.slope = act || a.col_sums;
-    const long cus = device_cus();
+    const long cus = real_cus();
     r.cut = slope_cut(a, cus);
     r.g_bytes = r.own_g ? up(a.m * a.n * s) : 0;
     r.s_bytes = a.col_sums && r.cut.parts > 1 ? up(r.cut.parts * std::max<long>(1, a.groups) * a.n * s) : 0;
@@ -585,7 +585,7 @@ Grad plan_grad(const locus_hip_product_grad_args& a)
         // both in one launch, tiles of one size, each with half the CUs; or one after the other (the second
         // launch comes about 4 us cheaper than the estimate of one alone)
         Want da = r.da, db = r.db;
-        da.cus = db.cus = cus / 2;
+        da.cus = db.cus = std::max<long>(1, cus / 2);
         da.tiles_only = db.tiles_only = true;
         Plan pa = plan_product(da), pb = plan_product(db);
         if (pa.tw != pb.tw) {
