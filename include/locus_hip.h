@@ -316,7 +316,9 @@ typedef struct locus_hip_product_args {
     const void* res; int64_t sr_m, sr_n;          /* or NULL; may be C (same strides)           */
     void* C; int64_t sc_m, sc_n;                  /* C and pre: rows (or columns) one behind the
                                                      other, sharing no memory with each other or
-                                                     with what is read (else LOCUS_HIP_EINVAL)   */
+                                                     with what is read (else LOCUS_HIP_EINVAL;
+                                                     views whose strides nest in no order, within
+                                                     each other's bounds, may count as sharing)  */
     void* pre; int64_t sp_m, sp_n;                /* or NULL: receives Z                        */
     int64_t groups; const int64_t* offsets;       /* [groups + 1]                               */
     int64_t sb_g, sbias_g;

@@ -391,7 +391,54 @@ struct Span {
                 const long gap = (((long)(o.at - at) + b0 - a0) % period + period) % period;
                 if (gap >= a1 - a0 && gap + (b1 - b0) <= period) return false;
             }
-        return true;
+        return common(o);
+    }
+    // Whether two of their elements share a byte: o.at - at + sum (o's steps) - sum (own steps), one term for each
+    // different stride, comes between -o.size and size.  The largest stride's multiples that the others can still
+    // bring there are few where strides are nested, as in views of one matrix; more than 4096 tries count as shared.
+    bool common(const Span& o) const
+    {
+        struct Term {
+            long step, lo, hi;
+        } t[6];
+        int terms = 0;
+        auto add = [&](long step, long lo, long hi) {
+            if (step == 0 || lo == hi) return;
+            if (step < 0) {
+                step = -step;
+                std::swap(lo, hi);
+                lo = -lo;
+                hi = -hi;
+            }
+            for (int q = 0; q < terms; ++q)
+                if (t[q].step == step) {
+                    t[q].lo += lo;
+                    t[q].hi += hi;
+                    return;
+                }
+            t[terms++] = {step, lo, hi};
+        };
+        for (int q = 0; q < 3; ++q) {
+            add(o.s[q], 0, o.n[q] - 1);
+            add(s[q], 1 - n[q], 0);
+        }
+        std::sort(t, t + terms, [](const Term& a, const Term& b) { return a.step > b.step; });
+        long lo[7] = {}, hi[7] = {};                     // what the terms from q on can add
+        for (int q = terms - 1; q >= 0; --q) {
+            lo[q] = lo[q + 1] + t[q].lo * t[q].step;
+            hi[q] = hi[q + 1] + t[q].hi * t[q].step;
+        }
+        auto floor_div = [](long a, long b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+        int tries = 0;
+        auto search = [&](auto&& self, int q, long sum) -> bool {
+            if (q == terms) return -o.size < sum && sum < size;
+            long x = std::max(t[q].lo, -floor_div(sum + hi[q + 1] + o.size - 1, t[q].step));
+            const long end = std::min(t[q].hi, floor_div(size - 1 - sum - lo[q + 1], t[q].step));
+            for (; x <= end; ++x)
+                if (++tries > 4096 || self(self, q + 1, sum + x * t[q].step)) return true;
+            return false;
+        };
+        return search(search, 0, (long)(o.at - at));
     }
 };
 
