@@ -470,7 +470,9 @@ int check_spans(const locus_hip_product_args& a)
         LOCUS_REQUIRE(!C.meets(r) && !pre.meets(r), "product: C or pre shares memory with what is read");
     LOCUS_REQUIRE(!C.meets(pre), "product: C shares memory with pre");
     LOCUS_REQUIRE(!pre.meets(res), "product: pre shares memory with the residual");
-    LOCUS_REQUIRE(!C.meets(res) || (a.C == a.res && a.sc_m == a.sr_m && a.sc_n == a.sr_n),
+    // (one row's or column's stride says nothing)
+    const bool same = a.C == a.res && (a.m == 1 || a.sc_m == a.sr_m) && (a.n == 1 || a.sc_n == a.sr_n);
+    LOCUS_REQUIRE(same || !C.meets(res),
                   "product: C shares memory with the residual and is not it");
     return 0;
 }

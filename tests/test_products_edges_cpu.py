@@ -79,3 +79,12 @@ def test_large_interleaved_views_end_quickly():
     for _ in range(50):
         shares(dict(m=1 << 20, n=64, k=1 << 16, sa_m=7919, sa_k=104729, B=1 << 45, sb_k=64, C=(1 << 20) + 8, sc_m=65, sc_n=1))
     assert time.perf_counter() - start < 1.0
+
+
+@pytest.mark.parametrize("kw,ok", [(dict(m=1, sr_m=77, sr_n=1), True), (dict(m=4, n=1, sc_m=3, sr_m=3, sr_n=5), True),
+                                   (dict(m=1, n=1, sr_m=0, sr_n=0), True), (dict(m=1, sr_m=77, sr_n=2), False),
+                                   (dict(m=4, sr_m=4, sr_n=1), False)])
+def test_one_row_in_place_of_its_residual(kw, ok):
+    """C is the residual; the stride of a single row or column, which a view may give any value, does not count."""
+    kw = dict(dict(n=3, k=64, sa_m=64, res=3 << 20), **kw)
+    assert shares(kw) != ok
