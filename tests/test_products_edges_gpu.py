@@ -28,3 +28,28 @@ def test_one_row_or_column_in_place_of_its_residual(pr, cfg):
         assert torch.equal(row, want)
         kept.view(-1)[3 * 70:3 * 70 + m * n] = want.reshape(-1)
         assert torch.equal(buf, kept)
+
+
+def test_callers_on_threads_of_their_own(pr):
+    """Two threads on their own streams, 20 calls each; what a thread raises fails the test."""
+    from concurrent.futures import ThreadPoolExecutor
+    A, B = normal(12, 70, 2003), normal(13, 2003, 65)
+    off = torch.tensor([0, 11, 70], device="cuda:0")
+    Bg, dC = torch.stack([B, 2 * B]), normal(14, 70, 65)
+    calls = [lambda: (pr.dense_product(A, B, act="gelu"), pr.grouped_product(A, Bg, off, cfg=(64, 2))),
+             lambda: pr.grouped_product_grad(dC, A, Bg, off, act="probit", pre=dC, need_bias=True)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+
+    def work(call, ref):
+        side, done = torch.cuda.Stream(), 0
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                got = call()
+                assert len(got) == len(ref) and all(torch.equal(g, w) for g, w in zip(got, ref))
+                done += 1
+        side.synchronize()
+        return done
+
+    with ThreadPoolExecutor(2) as pool:
+        assert [f.result() for f in [pool.submit(work, *x) for x in zip(calls, want)]] == [20, 20]
