@@ -14,7 +14,8 @@ log(1 + e^z), "gelu" z Phi(z) or "silu" z / (1 + e^-z).  float64 (the package's 
 sums are in that type and in a fixed order, so a call gives the same bits every time.  Any strides; one
 contiguous index per matrix is fast.  The calls are queued on the current stream of the tensors' device
 and return without waiting; outputs and workspaces come from torch's allocator, so the calls can be
-captured into a HIP graph.  They are outside autograd: gradients are the explicit calls here.
+captured into a HIP graph.  They are outside autograd: gradients are the explicit calls here, and tensors that
+require grad are refused unless under torch.no_grad().
 
 `offsets` (groups + 1 int64) and `gather` (int64) stay on the GPU and are not read by the host.  Whatever
 they hold, nothing out of bounds is touched: an offset counts as the largest of 0 and those before it, at
@@ -38,9 +39,13 @@ def _fail(msg):
 
 
 def _plain(name, t):
-    """Memory holds the values themselves (a conjugate's imaginary part, say, is kept with its sign pending)."""
+    """Memory holds the values themselves (a conjugate's imaginary part, say, is kept with its sign pending), and no
+    gradient is asked for, which would be lost here."""
     if t.is_neg():
         _fail(f"{name} is a negated view: pass {name}.resolve_neg()")
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail(f"{name} requires grad and the products are outside autograd: call them under torch.no_grad() or pass "
+              f"{name}.detach(); gradients are dense_product_grad and grouped_product_grad")
 
 
 def _check(name, t, like, shape):

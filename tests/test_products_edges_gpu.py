@@ -53,3 +53,31 @@ def test_callers_on_threads_of_their_own(pr):
 
     with ThreadPoolExecutor(2) as pool:
         assert [f.result() for f in [pool.submit(work, *x) for x in zip(calls, want)]] == [20, 20]
+
+
+def test_tensors_that_require_grad_are_refused(pr):
+    """The products are outside autograd: a result cut off from the graph would lose its gradient without a word.
+    Detached, or under no_grad, the same calls are made."""
+    A, B, off = normal(1, 4, 5), normal(2, 5, 3), torch.tensor([0, 1, 4], device="cuda:0")
+    bias, res, pre, dC = normal(3, 3), normal(4, 4, 3), normal(5, 4, 3), normal(6, 4, 3)
+
+    def dense(A=A, B=B, bias=bias, residual=res, out=None, pre=pre):
+        return pr.dense_product(A, B, bias=bias, residual=residual, out=out, pre=pre)
+
+    def grouped(A=A, B=B, bias=bias, residual=res):
+        return pr.grouped_product(A, torch.stack([B.detach(), B.detach()]).requires_grad_(B.requires_grad), off,
+                                  bias=torch.stack([bias.detach()] * 2).requires_grad_(bias.requires_grad), residual=residual)
+
+    def grad(A=A, B=B, dC=dC, pre=pre):
+        return pr.dense_product_grad(dC, A, B, act="silu", pre=pre, bias_grad="row")[0]
+
+    all_args = dict(A=A, B=B, bias=bias, residual=res, out=torch.zeros_like(res), pre=pre, dC=dC)
+    for fn in (dense, grouped, grad):
+        want = fn()
+        for name in fn.__code__.co_varnames[:fn.__code__.co_argcount]:
+            leaf = all_args[name].clone().requires_grad_()
+            with pytest.raises(ValueError, match=f"{name} requires grad.*no_grad"):
+                fn(**{name: leaf})
+            with torch.no_grad():
+                assert torch.equal(fn(**{name: leaf}), want)
+            assert torch.equal(fn(**{name: leaf.detach()}), want)
