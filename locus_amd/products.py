@@ -123,8 +123,12 @@ def _run(pack, run, fields, dev):
         _lib.check(rc)
 
 
-def _forward(fields, dev):
+def _forward(fields, dev, *given):
+    """given: tensors of the caller (or None) that the call writes to, which autograd is told."""
     _run(_ARGS.pack, _lib.lib().locus_hip_product_dev, fields, dev)
+    for t in given:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
 
 
 def _at(t):
@@ -174,10 +178,12 @@ def dense_product(A, B, bias=None, act="identity", residual=None, alpha=1.0, bet
     n = B.shape[1]
     code = _act(act)
     sbias = _bias_strides(bias, A, m, n) if bias is not None else (0, 0)
+    given = out
     out = _outputs(A, m, n, out, pre, residual)
     if m and n:
         _forward((m, n, k, dtype, code, _DENSE, 0, *cfg, alpha, beta, A.data_ptr(), *A.stride(), B.data_ptr(),
-                  *B.stride(), _ptr(bias), *sbias, *_at(residual), *_at(out), *_at(pre), 0, 0, 0, 0, 0, 0), A.device)
+                  *B.stride(), _ptr(bias), *sbias, *_at(residual), *_at(out), *_at(pre), 0, 0, 0, 0, 0, 0), A.device,
+                 given, pre)
     return out
 
 
@@ -193,14 +199,14 @@ def grouped_product(A, B, offsets, bias=None, act="identity", residual=None, alp
     code = _act(act)
     if bias is not None:
         _check("bias", bias, A, (groups, n))
-    fill = out is None
+    given, fill = out, out is None
     out = _outputs(A, m, n, out, pre, residual)
     if m and n:
         sb = B.stride()
         sbias = bias.stride() if bias is not None else (0, 0)
         _forward((m, n, k, dtype, code, _ROWS, fill, *cfg, alpha, beta, A.data_ptr(), *A.stride(), B.data_ptr(), sb[1],
                   sb[2], _ptr(bias), 0, sbias[1], *_at(residual), *_at(out), *_at(pre), groups, offsets.data_ptr(),
-                  sb[0], sbias[0], _ptr(gather), A.shape[0]), A.device)
+                  sb[0], sbias[0], _ptr(gather), A.shape[0]), A.device, given, pre)
     return out
 
 

@@ -81,3 +81,26 @@ def test_tensors_that_require_grad_are_refused(pr):
             with torch.no_grad():
                 assert torch.equal(fn(**{name: leaf}), want)
             assert torch.equal(fn(**{name: leaf.detach()}), want)
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("arg", ["out", "pre"])
+def test_autograd_sees_what_was_overwritten(pr, arg, grouped):
+    """A tensor that a graph of autograd holds for its backward pass, given as out or pre: the pass fails, as after any
+    operation in place, instead of using the new values."""
+    A, B, off = normal(1, 4, 5), normal(2, 5, 3), torch.tensor([0, 1, 4], device="cuda:0")
+    held, other = normal(3, 4, 3), normal(4, 4, 3)
+    leaf = torch.ones((4, 3), dtype=torch.float64, device="cuda:0", requires_grad=True)
+    y = (leaf * held).sum()
+    kw = {arg: held, "pre" if arg == "out" else "out": other}
+    before = other._version
+    if grouped:
+        pr.grouped_product(A, torch.stack([B, B]), off, **kw)
+    else:
+        pr.dense_product(A, B, **kw)
+    assert other._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():                    # tensors without a version
+        kw = {name: torch.empty_like(t) for name, t in kw.items()}
+        pr.dense_product(A, B, **kw)
