@@ -290,9 +290,13 @@ int locus_hip_gemm_dev(int64_t m, int64_t n, int64_t k, double alpha, const doub
  *           its own fit (fold, cohort, tissue).  Runs may be empty; rows before the first and behind
  *           the last run are left as they were (fill_rest: become 0 in C and pre).  gather: row r
  *           reads A's row gather[r] (the same row any number of times); C's rows are not moved.
+           Up to 65535 runs, meant for hundreds: every wave looks its run up among all of them
+           (65535 rows x 64 x 64 float32: in up to 257 runs 22 to 26 us, 1000 42 us, 4000 0.24 ms,
+           16000 2.7 ms, 65535 29 ms; the gradient 1.6 times that).
  * offsets and gather are device arrays, never read by the host.  Whatever they hold, nothing out of
  * bounds is touched: an offset counts as the largest of 0 and those before it, at most the number of
- * rows, and a gathered index outside [0, a_rows) makes its row NaN (in a gradient: its run's dB). */
+ * rows, and a gathered index outside [0, a_rows) makes its row NaN (in a gradient: its run's dB),
+ * unless k is 0 and nothing is gathered. */
 #define LOCUS_HIP_F64 0
 #define LOCUS_HIP_F32 1
 #define LOCUS_HIP_ACT_IDENTITY 0    /* z                                                        */

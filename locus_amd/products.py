@@ -193,8 +193,9 @@ def grouped_product(A, B, offsets, bias=None, act="identity", residual=None, alp
     offsets[g] <= r < offsets[g + 1]; src(r) = gather[r], or r without gather.
 
     B (groups x k x n), bias (groups x n).  C has as many rows as `gather`, else as A; they are in the order of
-    the runs (gathered rows are not moved back).  Runs may be empty.  Rows of no run are 0 in an `out` that
-    is made here, and are left as they were in one that is given (and in its `pre`)."""
+    the runs (gathered rows are not moved back).  Runs may be empty; they are meant to be hundreds (1000 cost
+    twice the time of few, many thousands milliseconds: see include/locus_hip.h).  Rows of no run are 0 in an
+    `out` that is made here, and are left as they were in one that is given; `pre` goes with `out`."""
     dtype, m, n, k, groups = _grouped_sizes(A, B, offsets, gather)
     code = _act(act)
     if bias is not None:

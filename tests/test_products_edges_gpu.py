@@ -104,3 +104,32 @@ def test_autograd_sees_what_was_overwritten(pr, arg, grouped):
     with torch.inference_mode():                    # tensors without a version
         kw = {name: torch.empty_like(t) for name, t in kw.items()}
         pr.dense_product(A, B, **kw)
+
+
+def test_as_many_runs_as_there_may_be(pr):
+    """65 535 runs, empty ones among them, rows of no run before and behind.  Sums of k and of a run's rows in float64:
+    2 (terms + 4) 2^-53 of the terms' magnitudes."""
+    rng = np.random.default_rng(20)
+    gr, m, k, n = 65535, 70000, 3, 2
+    off = np.sort(rng.integers(5, m - 7, size=gr + 1))
+    A, B, dC = rng.normal(size=(m, k)), rng.normal(size=(gr, k, n)), rng.normal(size=(m, n))
+    run = np.searchsorted(off, np.arange(m), side="right") - 1
+    rows = (run >= 0) & (run < gr)
+    g = np.clip(run, 0, gr - 1)
+    u, most = 2.0 ** -53, np.diff(off).max()
+
+    def close(got, want, terms, count):
+        assert (np.abs(got.cpu().numpy() - want) <= 2 * (count + 4) * u * terms).all()
+
+    up = [torch.from_numpy(x).to("cuda:0") for x in (A, B, off)]
+    for cfg in ((0, 0), (64, 1)):
+        P = np.einsum("mk,mkn->mn", A, B[g]) * rows[:, None]
+        close(pr.grouped_product(*up, cfg=cfg), P, np.einsum("mk,mkn->mn", np.abs(A), np.abs(B[g])) * rows[:, None], k)
+        dA, dB, db = pr.grouped_product_grad(torch.from_numpy(dC).to("cuda:0"), *up, need_bias=True, cfg=cfg)
+        close(dA, np.einsum("mn,mkn->mk", dC, B[g]) * rows[:, None],
+              np.einsum("mn,mkn->mk", np.abs(dC), np.abs(B[g])) * rows[:, None], n)
+        for got, each in ((dB, A[:, :, None] * dC[:, None]), (db, dC)):
+            want, terms = np.zeros((gr, *each.shape[1:])), np.zeros((gr, *each.shape[1:]))
+            np.add.at(want, run[rows], each[rows])
+            np.add.at(terms, run[rows], np.abs(each[rows]))
+            close(got, want, terms, most)
