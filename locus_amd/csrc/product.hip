@@ -157,10 +157,11 @@ struct Want {
 
 // Which kernel, tile and split: the quickest by the estimates below, whose constants are fitted to measurements: 350
 // products of 1 .. 4000 rows, 20 .. 20 000 covariates and 1 .. 10 000 columns, alone or in up to 100 runs, in 26
-// geometries each, replayed from a graph.  The estimate's choice took 2 to 3 % longer than the best of them in either
-// type (rows up to 48 by the kernel for few, the rest in tiles: 12 % longer).
+// geometries each, replayed from a graph.  On 200 others (profiles/products_plan.csv) its choice took 5 % longer than
+// the best geometry for one pair, 8 for runs, 2 and 3 for gradients, where that one takes over 20 us.
 //   Joining a split sum: 2.4 us, and the partials written and read at 4.2 TB/s.  Called one by one, a workspace and
-// another launch cost the host more than that (host_us).
+// another launch cost the host more than that (host_us), so short calls are not split.  Replayed from a graph they
+// would gain by it, 8 us against 14 at most (over all of those sizes 13, 10, 6 and 2 %): such a caller names a geometry.
 //   Few rows: 5.1 us, 1.2 for every round of two workgroups a CU, C and what goes with it at 9 TB/s, and the longer of:
 // a wave's blocks of k, 0.36 us each, times the workgroups a CU has; what they read through L2 at 7.6 TB/s (by the
 // root of what the last round leaves idle longer).

@@ -8,7 +8,7 @@
 // does its TW x TW matrix instructions, so that they wait for no read just issued.  LDS rows are 15 elements
 // longer than the tile: odd, so that the transposing stores of an operand whose contiguous index is k spread
 // over the banks, and small enough that tiles of 64 (40 KB) fit a CU four times, tiles of 128 (74 KB) twice.
-// Those four keep its matrix cores 90 % busy (2000 x 20 000 x 500 float64; 79 % in the two products of a gradient,
+// Those four keep its matrix cores 90 % busy (2000 x 20 000 x 500 float64; 84 % in the two products of a gradient,
 // 1999 x 5000 x 1000 float32); one alone reaches 67 % of the rate.  Tiles of 128 read half as much and are chosen
 // where the sums are long and the tiles fill the chip evenly.
 //
