@@ -32,6 +32,9 @@ def _raw_effects(eff, A, rmvd):
         raise ValueError("the training covariates do not go with the fit: "
                          f"{len(keep)} columns kept, {eff.shape[0]} rows of effects")
     mean, sd = A.mean(axis=0)[keep], A.std(axis=0, ddof=1)[keep]
+    if not sd.all():
+        raise ValueError("the training covariates do not go with the fit: kept columns of one value: "
+                         f"{keep[sd == 0].tolist()}")
     flat = (A.max(axis=0) == A.min(axis=0))[keep]
     const = ((A[0, keep] - mean) / sd)[flat] @ eff[flat]
     out = np.zeros((A.shape[1], eff.shape[1]))

@@ -25,3 +25,15 @@ def test_columns_of_one_value(order, value):
         same[:, 2] = value
         assert np.abs((new - same) @ out).max() == 0
     assert kept or value in (2.0, 0.0)
+
+
+def test_a_kept_column_without_deviation_is_refused():
+    """The fit cannot have kept it: these are not the covariates it was given (predictions would be NaN)."""
+    from locus_amd import Predictor
+    X = np.random.default_rng(0).normal(size=(20, 4))
+    X[:, 1] = 2.0
+    vb = dict(beta_vb=np.ones((4, 2)), alpha_vb=np.zeros((2, 2)), rmvd_x=np.array([], dtype=int))
+    with pytest.raises(ValueError, match="do not go with the fit.*1"):
+        Predictor(dict(vb, alpha_vb=np.zeros((1, 2))), X, link="probit")
+    with pytest.raises(ValueError, match="do not go with the fit.*0"):
+        Predictor(vb, np.random.default_rng(1).normal(size=(20, 4)), Z=np.ones((20, 1)), link="probit")
